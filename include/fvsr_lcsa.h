@@ -336,6 +336,69 @@ fvsr_status fvsr_rmsnorm(int32_t m, int32_t c, const void* x, const void* weight
 fvsr_status fvsr_cross_attention(int32_t heads, int32_t lq, int32_t lk, const void* q, const void* k, const void* v,
                                  void* out, fvsr_stream_t stream);
 
+/* ---- 8-bit tensors: e4m3 values with a power-of-two scale for each block of 128 ----
+ * The form activations are kept in between a forward and a backward pass, and the operands of fvsr_linear_fp8. A (rows,
+ * cols) tensor is held as
+ *   values  e4m3, rows of ld = cols rounded up to 128 bytes, padding zero: rows * ld bytes;
+ *   scales  8-bit codes, one for each block of 128 values along a row: value = e4m3 * 2^(code - 127). The 128 rows x 4
+ *           blocks of a tile are 512 bytes; row r's code of block b is at (r % 32) * 16 + (r % 128) / 32 * 4 + b % 4 of
+ *           tile (r / 128, b / 4), tiles row-major: ceil(rows / 128) * ceil(cols / 512) * 512 bytes.
+ * A block's code is the smallest, at least 0, at which every magnitude is at most 448 * 2^(code - 127); values are then
+ * rounded to e4m3, to nearest with ties to even (off by at most 2^-4 of the value, or 2^-10 of the block's scale below
+ * e4m3's normal range). A block that holds an infinity or a NaN has code 255 and reads back as NaN throughout.
+ *
+ * fvsr_fp8_bytes — the two sizes for (rows, cols); either pointer may be NULL.
+ * fvsr_quantize_fp8 — x (rows, cols), dtype FVSR_BF16 or FVSR_F32, into its form (q, scale) and / or the form of its
+ * transpose, a (cols, rows) tensor (qt, scale_t); a pair may be NULL, not both. square = 0: one scale for each row's
+ * block (of x for q, of its transpose for qt); 1: one for each 128 x 128 square of x, the same for both forms (weights).
+ * fvsr_dequantize_fp8 — the values back as bf16 or fp32 (rounded once; exact unless below bf16's / fp32's range).
+ * rows >= 0, 1 <= cols, rows and cols at most 2^30, rows * cols at most 2^40. 16-byte alignment for x, q, qt and the
+ * scales; 4-byte for the tensor read back into. */
+fvsr_status fvsr_fp8_bytes(int64_t rows, int64_t cols, size_t* value_bytes, size_t* scale_bytes);
+fvsr_status fvsr_quantize_fp8(int64_t rows, int64_t cols, const void* x, int32_t dtype, int32_t square, void* q,
+                              void* scale, void* qt, void* scale_t, fvsr_stream_t stream);
+fvsr_status fvsr_dequantize_fp8(int64_t rows, int64_t cols, const void* q, const void* scale, void* out, int32_t dtype,
+                                fvsr_stream_t stream);
+
+/* ---- Linear layers on 8-bit operands ----
+ * fvsr_linear_fp8 — out = epilogue(x . w^T + bias): x (m, k) and w (n, k) in the 8-bit form, or, with x_scale NULL, x
+ * (m, k) bf16, which the call quantises first (one scale for each row's block of 128). Any m >= 0 (0: nothing to do),
+ * n, k >= 1. The same call is a layer's forward pass (w with square blocks or rows'), its input gradient (dy and the
+ * transposed w), its weight gradient (the transposed forms of dy and x; out FVSR_F32) and the single token's (m = 1).
+ * epilogue: fvsr_linear_epilogue, in fp32 with one rounding at the end: GELU(tanh) of the linear, or resid + gate *
+ * linear. bias and gate (n) bf16 (bias may be NULL); out and resid (m, n) of out_dtype (resid may be out, else they do
+ * not overlap). fp32 sums. workspace: fvsr_linear_fp8_workspace_size bytes (may be 0), 16-byte aligned, for this call
+ * alone until it is done. m, n, k at most 2^22, each tensor at most 2^40 bytes. 16-byte alignment for x, w and the
+ * scales, 4-byte for out and resid, 2-byte for bias and gate. */
+fvsr_status fvsr_linear_fp8_workspace_size(int32_t m, int32_t n, int32_t k, int32_t x_is_fp8, size_t* bytes);
+fvsr_status fvsr_linear_fp8(int32_t m, int32_t n, int32_t k, const void* x, const void* x_scale, const void* w,
+                            const void* w_scale, const void* bias, int32_t epilogue, const void* gate,
+                            const void* resid, void* out, int32_t out_dtype, void* workspace, size_t workspace_bytes,
+                            fvsr_stream_t stream);
+
+/* ---- LayerNorm for training ----
+ * fvsr_layernorm_train — the forward pass over c channels (1 to 8192, any number) of each of m rows that keeps what the
+ * backward pass needs: mean and rstd = 1 / sqrt(var + eps) (m fp32 each). n = (x - mean) * rstd, out = (n * weight +
+ * bias) * (1 + scale) + shift; weight and bias, and shift and scale, are given together or not at all, and both pairs
+ * may be. x, out and the vectors in dtype (FVSR_BF16 or FVSR_F32); fp32 arithmetic, out rounded once (fvsr_layernorm
+ * keeps the reference's rounding points instead). out may be x.
+ * fvsr_layernorm_backward — dx and the vectors' gradients (fp32, (c); each may be NULL) from dy, mean and rstd and the
+ * input x: in dtype with x_scale NULL, or in the 8-bit form. With g = dy * (1 + scale) * weight: dx = rstd * (g -
+ * mean_c(g) - n * mean_c(g * n)); dweight = (1 + scale) * sum(dy * n), dbias = (1 + scale) * sum(dy), dscale =
+ * sum(dy * (n * weight + bias)), dshift = sum(dy), sums over the rows in a fixed order (the same bits each time). dx may
+ * be dy. weight, bias and scale as in the forward pass (shift is not needed). workspace:
+ * fvsr_layernorm_backward_workspace_size bytes, 16-byte aligned, for this call alone until it is done. With m = 0 the
+ * vectors' gradients are zero. Alignment: a row-major tensor needs its element's (8-bit values and scales: 16). */
+fvsr_status fvsr_layernorm_train(int64_t m, int32_t c, const void* x, int32_t dtype, const void* weight,
+                                 const void* bias, const void* shift, const void* scale, float eps, void* out,
+                                 float* mean, float* rstd, fvsr_stream_t stream);
+fvsr_status fvsr_layernorm_backward_workspace_size(int64_t m, int32_t c, size_t* bytes);
+fvsr_status fvsr_layernorm_backward(int64_t m, int32_t c, const void* dy, int32_t dtype, const void* x,
+                                    const void* x_scale, const float* mean, const float* rstd, const void* weight,
+                                    const void* bias, const void* scale, void* dx, float* dweight, float* dbias,
+                                    float* dscale, float* dshift, void* workspace, size_t workspace_bytes,
+                                    fvsr_stream_t stream);
+
 /* ---- Streaming driver: the LCSA side of FlashVSR's chunk loop ----
  * Mirrors FlashVSRPipeline.chunk / FlashVSRDiT.step (Pipeline.swift:95-102, 112-131; DiT.swift:472-485, 554-578) for
  * the self-attention of `layers` DiT blocks at an output size out_h × out_w (multiples of 128; spatial blocks

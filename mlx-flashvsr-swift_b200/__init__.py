@@ -40,7 +40,9 @@ EXPORTED = [
     "fvsr_stream_workspace_size", "fvsr_stream_start_chunk", "fvsr_stream_rope", "fvsr_stream_layer",
     "fvsr_kv_cache_create_padded", "fvsr_kv_cache_reserve", "fvsr_kv_cache_commit", "fvsr_lcsa_forward_shard",
     "fvsr_lcsa_partial_size", "fvsr_lcsa_select_shard", "fvsr_lcsa_attend_shard", "fvsr_linear", "fvsr_linear_qkv",
-    "fvsr_layernorm", "fvsr_rmsnorm", "fvsr_cross_attention",
+    "fvsr_layernorm", "fvsr_rmsnorm", "fvsr_cross_attention", "fvsr_fp8_bytes", "fvsr_quantize_fp8",
+    "fvsr_dequantize_fp8", "fvsr_linear_fp8_workspace_size", "fvsr_linear_fp8", "fvsr_layernorm_train",
+    "fvsr_layernorm_backward_workspace_size", "fvsr_layernorm_backward",
 ]
 
 
@@ -130,6 +132,14 @@ def lib() -> ctypes.CDLL:
         "fvsr_layernorm": ([I32, I32, P, P, P, P, P, ctypes.c_float, P, P], ctypes.c_int),
         "fvsr_rmsnorm": ([I32, I32, P, P, ctypes.c_float, P, P], ctypes.c_int),
         "fvsr_cross_attention": ([I32, I32, I32, P, P, P, P, P], ctypes.c_int),
+        "fvsr_fp8_bytes": ([I64, I64, ctypes.POINTER(SZ), ctypes.POINTER(SZ)], ctypes.c_int),
+        "fvsr_quantize_fp8": ([I64, I64, P, I32, I32, P, P, P, P, P], ctypes.c_int),
+        "fvsr_dequantize_fp8": ([I64, I64, P, P, P, I32, P], ctypes.c_int),
+        "fvsr_linear_fp8_workspace_size": ([I32, I32, I32, I32, ctypes.POINTER(SZ)], ctypes.c_int),
+        "fvsr_linear_fp8": ([I32, I32, I32, P, P, P, P, P, I32, P, P, P, I32, P, SZ, P], ctypes.c_int),
+        "fvsr_layernorm_train": ([I64, I32, P, I32, P, P, P, P, ctypes.c_float, P, P, P, P], ctypes.c_int),
+        "fvsr_layernorm_backward_workspace_size": ([I64, I32, ctypes.POINTER(SZ)], ctypes.c_int),
+        "fvsr_layernorm_backward": ([I64, I32, P, I32, P, P, P, P, P, P, P, P, P, P, P, P, P, SZ, P], ctypes.c_int),
     }
     for name, (args, res) in sigs.items():
         fn = getattr(L, name)
@@ -701,6 +711,246 @@ def cross_attention(q, k, v, heads: int, out=None, stream=None):
     _check(lib().fvsr_cross_attention(int(heads), q.shape[0], k.shape[0], _ptr(q), _ptr(k), _ptr(v), _ptr(out),
                                       _stream(stream)))
     return out
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# 8-bit tensors, the linear layers on them, LayerNorm for training
+# ---------------------------------------------------------------------------------------------------------------
+
+class Fp8Tensor:
+    """A (rows, cols) tensor held in 8 bits (include/fvsr_lcsa.h, "8-bit tensors"): data (rows, cols rounded up to 128)
+    float8_e4m3fn, padding zero, and the e8m0 codes of its blocks of 128 in tiles, scale (ceil(rows / 128),
+    ceil(cols / 512), 512) uint8. Made by quantize_fp8; the constructor takes stored parts (a saved checkpoint)."""
+
+    __slots__ = ("data", "scale", "rows", "cols")
+
+    def __init__(self, data, scale, rows: int, cols: int):
+        torch = _torch()
+        if rows < 0 or cols < 1 or data.dtype != torch.float8_e4m3fn or scale.dtype != torch.uint8 or \
+                data.shape != (rows, (cols + 127) // 128 * 128) or \
+                scale.shape != ((rows + 127) // 128, (cols + 511) // 512, 512):
+            raise FVSRError(FVSR_EINVAL, f"not the stored parts of a ({rows}, {cols}) 8-bit tensor")
+        if not data.is_cuda or data.device != scale.device or not data.is_contiguous() or not scale.is_contiguous():
+            raise FVSRError(FVSR_EINVAL, "the parts of an 8-bit tensor must be contiguous on one CUDA device")
+        self.data, self.scale, self.rows, self.cols = data, scale, int(rows), int(cols)
+
+    @property
+    def device(self):
+        return self.data.device
+
+    @property
+    def shape(self):
+        return (self.rows, self.cols)
+
+    def codes(self):
+        """The blocks' codes (rows, ceil(cols / 128)) uint8, a view: a block's scale is 2^(code - 127)."""
+        rt, kt, _ = self.scale.shape
+        full = self.scale.view(rt, kt, 32, 4, 4).permute(0, 3, 2, 1, 4).reshape(rt * 128, kt * 4)
+        return full[:self.rows, :(self.cols + 127) // 128]
+
+    @staticmethod
+    def empty(rows: int, cols: int, device="cuda") -> "Fp8Tensor":
+        torch = _torch()
+        return Fp8Tensor(
+            torch.empty((rows, (cols + 127) // 128 * 128), dtype=torch.float8_e4m3fn, device=device),
+            torch.empty(((rows + 127) // 128, (cols + 511) // 512, 512), dtype=torch.uint8, device=device), rows, cols)
+
+
+class _Launch:
+    """`with _Launch(device, stream) as handle`: the device of the operands is current and the stream the launches go to
+    is the current one, so memory allocated inside belongs to that stream; handle is the stream's."""
+
+    __slots__ = ("device", "stream", "ctx")
+
+    def __init__(self, device, stream):
+        self.device, self.stream, self.ctx = device, stream, None
+
+    def __enter__(self):
+        torch = _torch()
+        if self.stream is not None:
+            if self.stream.device != self.device:
+                raise FVSRError(FVSR_EINVAL, f"the stream is on {self.stream.device}, the tensors on {self.device}")
+            self.ctx = torch.cuda.stream(self.stream)
+            self.ctx.__enter__()
+            return ctypes.c_void_p(self.stream.cuda_stream)
+        if torch.cuda.current_device() != self.device.index:
+            self.ctx = torch.cuda.device(self.device)
+            self.ctx.__enter__()
+        return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+    def __exit__(self, *exc):
+        if self.ctx is not None:
+            self.ctx.__exit__(*exc)
+        return False
+
+
+def _matrix(t, name, dtypes=None, shape=None, device=None):
+    """t as a contiguous 2-D CUDA tensor ((1, L, C) becomes (L, C)) of one of the dtypes, or FVSRError."""
+    torch = _torch()
+    if t.dim() == 3 and t.shape[0] == 1:
+        t = t[0]
+    if t.dim() != 2 or t.dtype not in (dtypes or (torch.bfloat16, torch.float32)) or not t.is_cuda or \
+            not t.is_contiguous():
+        raise FVSRError(FVSR_EINVAL, f"{name} must be a contiguous 2-D CUDA tensor, bfloat16 or float32 as the call allows")
+    if (shape is not None and tuple(t.shape) != shape) or (device is not None and t.device != device):
+        raise FVSRError(FVSR_EINVAL, f"{name} must be {shape} on {device}, got {tuple(t.shape)} on {t.device}")
+    return t
+
+
+def _channel_vector(t, name, n, dtype, device):
+    if t is not None and (t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or t.device != device or
+                          not t.is_contiguous()):
+        raise FVSRError(FVSR_EINVAL, f"{name} must be contiguous ({n},) {dtype} on {device}")
+    return t
+
+
+def quantize_fp8(x, square: bool = False, transpose: bool = False, out=None, stream=None) -> Fp8Tensor:
+    """x (rows, cols) bf16 or fp32 in its 8-bit form (fvsr_quantize_fp8): a power-of-two scale for each row's block of
+    128, or with square for each 128 x 128 square (weights). transpose: the form of x's transpose, (cols, rows), whose
+    blocks run along x's rows (the checkpoint a weight gradient reads)."""
+    x = _matrix(x, "x")
+    rows, cols = x.shape
+    with _Launch(x.device, stream) as st:
+        shape = (cols, rows) if transpose else (rows, cols)
+        if out is None:
+            out = Fp8Tensor.empty(*shape, device=x.device)
+        elif out.shape != shape or out.device != x.device:
+            raise FVSRError(FVSR_EINVAL, f"out must be an 8-bit tensor of {shape} on {x.device}")
+        held = (_ptr(out.data), _ptr(out.scale))
+        _check(lib().fvsr_quantize_fp8(rows, cols, _ptr(x), _dtype_code(x), int(bool(square)),
+                                       *((None, None) + held if transpose else held + (None, None)), st))
+    return out
+
+
+def quantize_fp8_both(x, square: bool = False, stream=None) -> tuple:
+    """(quantize_fp8(x), quantize_fp8(x, transpose=True)) from one pass over x."""
+    x = _matrix(x, "x")
+    rows, cols = x.shape
+    if rows == 0:
+        raise FVSRError(FVSR_EINVAL, "the transpose of a tensor without rows has no form")
+    with _Launch(x.device, stream) as st:
+        out, out_t = Fp8Tensor.empty(rows, cols, x.device), Fp8Tensor.empty(cols, rows, x.device)
+        _check(lib().fvsr_quantize_fp8(rows, cols, _ptr(x), _dtype_code(x), int(bool(square)), _ptr(out.data),
+                                       _ptr(out.scale), _ptr(out_t.data), _ptr(out_t.scale), st))
+    return out, out_t
+
+
+def dequantize_fp8(t: Fp8Tensor, dtype=None, out=None, stream=None):
+    """The values of an 8-bit tensor as bf16 (the default) or fp32 (fvsr_dequantize_fp8)."""
+    torch = _torch()
+    with _Launch(t.device, stream) as st:
+        if out is None:
+            out = torch.empty((t.rows, t.cols), dtype=dtype or torch.bfloat16, device=t.device)
+        out = _matrix(out, "out", shape=t.shape, device=t.device)
+        if dtype is not None and out.dtype != dtype:
+            raise FVSRError(FVSR_EINVAL, f"out must be {dtype}")
+        _check(lib().fvsr_dequantize_fp8(t.rows, t.cols, _ptr(t.data), _ptr(t.scale), _ptr(out), _dtype_code(out), st))
+    return out
+
+
+def linear_fp8(x, w: Fp8Tensor, bias=None, epilogue: int = FVSR_LINEAR, gate=None, resid=None, out=None,
+               out_dtype=None, workspace=None, stream=None):
+    """A linear layer on 8-bit operands (fvsr_linear_fp8): x (M, K) an Fp8Tensor, or bf16 and quantised in the call; w
+    (N, K) an Fp8Tensor; bias, gate (N) bf16; the epilogues of `linear` in fp32 with one rounding. out (M, N) bf16 (the
+    default) or fp32, resid like out. Input gradient: linear_fp8(dy, w_t) with w_t the transposed form of the weight;
+    weight gradient: linear_fp8(dy_t, x_t, out_dtype=torch.float32) with the transposed forms of dy and x. workspace:
+    a uint8 tensor of linear_fp8_workspace_size(...) bytes, else it is allocated."""
+    torch = _torch()
+    held = isinstance(x, Fp8Tensor)
+    if not held:
+        x = _matrix(x, "x", dtypes=(torch.bfloat16,))
+    if not isinstance(w, Fp8Tensor):
+        raise FVSRError(FVSR_EINVAL, "w must be an Fp8Tensor")
+    (m, k), n, dev = x.shape, w.rows, w.device
+    if w.cols != k or x.device != dev:
+        raise FVSRError(FVSR_EINVAL, f"w must be ({n}, {k}) on {x.device}")
+    _channel_vector(bias, "bias", n, torch.bfloat16, dev)
+    _channel_vector(gate, "gate", n, torch.bfloat16, dev)
+    if out is not None:
+        out = _matrix(out, "out", shape=(m, n), device=dev)
+        out_dtype = out_dtype or out.dtype
+    out_dtype = out_dtype or torch.bfloat16
+    if out is not None and out.dtype != out_dtype:
+        raise FVSRError(FVSR_EINVAL, f"out must be {out_dtype}")
+    if resid is not None:
+        resid = _matrix(resid, "resid", dtypes=(out_dtype,), shape=(m, n), device=dev)
+    with _Launch(dev, stream) as st:
+        if out is None:
+            if out_dtype not in (torch.bfloat16, torch.float32):
+                raise FVSRError(FVSR_EINVAL, f"out must be bfloat16 or float32, got {out_dtype}")
+            out = torch.empty((m, n), dtype=out_dtype, device=dev)
+        need = linear_fp8_workspace_size(m, n, k, held) if workspace is None else 0
+        if need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        xp, xs = (_ptr(x.data), _ptr(x.scale)) if held else (_ptr(x), None)
+        _check(lib().fvsr_linear_fp8(m, n, k, xp, xs, _ptr(w.data), _ptr(w.scale), _ptr(bias), int(epilogue),
+                                     _ptr(gate), _ptr(resid), _ptr(out), _dtype_code(out), _ptr(workspace),
+                                     0 if workspace is None else workspace.numel(), st))
+    return out
+
+
+def linear_fp8_workspace_size(m: int, n: int, k: int, x_is_fp8: bool) -> int:
+    size = ctypes.c_size_t(0)
+    _check(lib().fvsr_linear_fp8_workspace_size(m, n, k, int(x_is_fp8), ctypes.byref(size)))
+    return size.value
+
+
+def layernorm_train(x, weight=None, bias=None, shift=None, scale=None, eps: float = 1e-6, out=None, stream=None):
+    """LayerNorm's forward pass for training (fvsr_layernorm_train): (out, mean, rstd) with n = (x - mean) * rstd and
+    out = (n * weight + bias) * (1 + scale) + shift; x (M, C) bf16 or fp32, the vectors (C) like x, mean and rstd (M)
+    fp32 for layernorm_backward."""
+    torch = _torch()
+    x = _matrix(x, "x")
+    m, c = x.shape
+    for t, name in ((weight, "weight"), (bias, "bias"), (shift, "shift"), (scale, "scale")):
+        _channel_vector(t, name, c, x.dtype, x.device)
+    if out is not None:
+        out = _matrix(out, "out", dtypes=(x.dtype,), shape=(m, c), device=x.device)
+    with _Launch(x.device, stream) as st:
+        if out is None:
+            out = torch.empty_like(x)
+        mean, rstd = torch.empty((2, m), dtype=torch.float32, device=x.device).unbind(0)
+        _check(lib().fvsr_layernorm_train(m, c, _ptr(x), _dtype_code(x), _ptr(weight), _ptr(bias), _ptr(shift),
+                                          _ptr(scale), float(eps), _ptr(out), _ptr(mean), _ptr(rstd), st))
+    return out, mean, rstd
+
+
+def layernorm_backward(dy, x, mean, rstd, weight=None, bias=None, scale=None, dx=None, workspace=None, stream=None):
+    """LayerNorm's backward pass (fvsr_layernorm_backward): x the forward's input, in dy's dtype or as an Fp8Tensor (its
+    8-bit form); weight, bias and scale as the forward had them. Returns {"dx", "dweight", "dbias", "dscale",
+    "dshift"}: dx (M, C) like dy, the vectors' gradients (C) fp32, None where the forward had no such vector."""
+    torch = _torch()
+    dy = _matrix(dy, "dy")
+    m, c = dy.shape
+    dev = dy.device
+    held = isinstance(x, Fp8Tensor)
+    if held:
+        if x.shape != (m, c) or x.device != dev:
+            raise FVSRError(FVSR_EINVAL, f"x must be ({m}, {c}) on {dev}")
+    else:
+        x = _matrix(x, "x", dtypes=(dy.dtype,), shape=(m, c), device=dev)
+    _channel_vector(mean, "mean", m, torch.float32, dev)
+    _channel_vector(rstd, "rstd", m, torch.float32, dev)
+    for t, name in ((weight, "weight"), (bias, "bias"), (scale, "scale")):
+        _channel_vector(t, name, c, dy.dtype, dev)
+    if dx is not None:
+        dx = _matrix(dx, "dx", dtypes=(dy.dtype,), shape=(m, c), device=dev)
+    with _Launch(dev, stream) as st:
+        if dx is None:
+            dx = torch.empty_like(dy)
+        kinds = (["dweight", "dbias"] if weight is not None else []) + (["dscale", "dshift"] if scale is not None else [])
+        grads = dict(zip(kinds, torch.empty((len(kinds), c), dtype=torch.float32, device=dev).unbind(0))) if kinds else {}
+        if workspace is None:
+            size = ctypes.c_size_t(0)
+            _check(lib().fvsr_layernorm_backward_workspace_size(m, c, ctypes.byref(size)))
+            workspace = torch.empty(size.value, dtype=torch.uint8, device=dev) if size.value else None
+        g = {k: grads.get(k) for k in ("dweight", "dbias", "dscale", "dshift")}
+        xp, xs = (_ptr(x.data), _ptr(x.scale)) if held else (_ptr(x), None)
+        _check(lib().fvsr_layernorm_backward(m, c, _ptr(dy), _dtype_code(dy), xp, xs, _ptr(mean), _ptr(rstd),
+                                             _ptr(weight), _ptr(bias), _ptr(scale), _ptr(dx), _ptr(g["dweight"]),
+                                             _ptr(g["dbias"]), _ptr(g["dscale"]), _ptr(g["dshift"]), _ptr(workspace),
+                                             0 if workspace is None else workspace.numel(), st))
+    return {"dx": dx, **g}
 
 
 def rope_tables(f: int, h: int, w: int, t0: int = 0, head_dim: int = 128, theta: float = 10000.0, device="cuda"):

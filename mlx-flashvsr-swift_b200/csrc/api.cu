@@ -13,6 +13,7 @@
 
 namespace fvsr {
 void set_last_error(const char* msg);
+int current_device_is_sm100(int* dev);
 }
 
 using namespace fvsr;
@@ -277,6 +278,13 @@ fvsr_status check_prepare_inputs(const fvsr_lcsa_params* p, const Dims& d, const
 }
 
 }  // namespace
+
+// check_device_sm100 for the entry points of other files: whether the current device (*dev) is an sm_100 part.
+int fvsr::current_device_is_sm100(int* dev) {
+    *dev = -1;
+    cudaGetDevice(dev);
+    return check_device_sm100() == FVSR_OK;
+}
 
 extern "C" {
 
