@@ -62,6 +62,20 @@ fvsr_status check_linear_shape(int32_t m, int32_t n, int32_t k) {
     return FVSR_OK;
 }
 
+// The workspace of a linear layer: the 8-bit form of a bf16 x, then the partial products of a sum over K in parts.
+struct LinearWorkspace {
+    size_t scale, partial, bytes;
+    Fp8GemmPlan plan;
+};
+LinearWorkspace linear_workspace(int m, int n, int k, bool x_is_fp8) {
+    LinearWorkspace w;
+    w.plan = plan_gemm_fp8(m, n, k);
+    w.scale = x_is_fp8 ? 0 : up256((size_t)(m * fp8_ld(k)));
+    w.partial = x_is_fp8 ? 0 : w.scale + up256((size_t)fp8_scale_bytes(m, k));
+    w.bytes = w.partial + up256(w.plan.partial_bytes);
+    return w;
+}
+
 fvsr_status check_norm(int64_t m, int32_t c, int32_t dtype) {
     if (m < 0 || c < 1) return refuse(FVSR_EINVAL, "layernorm: m must be >= 0 and c >= 1, got %lld and %d", (long long)m, c);
     if (c > kNormTrainMaxC) return refuse(FVSR_EUNSUPPORTED, "layernorm: c must be at most %d, got %d", kNormTrainMaxC, c);
@@ -116,7 +130,7 @@ fvsr_status fvsr_linear_fp8_workspace_size(int32_t m, int32_t n, int32_t k, int3
     fvsr_status s = check_linear_shape(m, n, k);
     if (s != FVSR_OK) return s;
     if (!bytes) return refuse(FVSR_EINVAL, "bytes is NULL");
-    *bytes = m == 0 || x_is_fp8 ? 0 : up256((size_t)(m * fp8_ld(k))) + up256((size_t)fp8_scale_bytes(m, k));
+    *bytes = m == 0 ? 0 : linear_workspace(m, n, k, x_is_fp8 != 0).bytes;
     return FVSR_OK;
 }
 
@@ -135,8 +149,8 @@ fvsr_status fvsr_linear_fp8(int32_t m, int32_t n, int32_t k, const void* x, cons
     if (!aligned(x, 16) || !aligned(x_scale, 16) || !aligned(w, 16) || !aligned(w_scale, 16) || !aligned(out, 4) ||
         !aligned(resid, 4) || !aligned(bias, 2) || !aligned(gate, 2))
         return refuse(FVSR_EINVAL, "x, w and the scales must be 16-byte aligned, out and resid 4-byte, bias and gate 2-byte aligned");
-    size_t need = 0;
-    if ((s = fvsr_linear_fp8_workspace_size(m, n, k, x_scale != nullptr, &need)) != FVSR_OK) return s;
+    const LinearWorkspace ws = linear_workspace(m, n, k, x_scale != nullptr);
+    const size_t need = ws.bytes;
     if (need > 0 && !workspace) return refuse(FVSR_EINVAL, "the workspace is required");
     if (workspace_bytes < need)
         return refuse(FVSR_ENOMEM, "workspace of %zu bytes is smaller than the %zu required", workspace_bytes, need);
@@ -149,7 +163,7 @@ fvsr_status fvsr_linear_fp8(int32_t m, int32_t n, int32_t k, const void* x, cons
     a.x_scale = static_cast<const uint8_t*>(x_scale);
     if (!x_scale) {
         uint8_t* q = static_cast<uint8_t*>(workspace);
-        uint8_t* scale = q + up256((size_t)(m * fp8_ld(k)));
+        uint8_t* scale = q + ws.scale;
         s = launched(launch_quantize_fp8(m, k, x, FVSR_BF16, false, q, scale, nullptr, nullptr, st), "quantize launch");
         if (s != FVSR_OK) return s;
         a.x = q, a.x_scale = scale;
@@ -162,7 +176,8 @@ fvsr_status fvsr_linear_fp8(int32_t m, int32_t n, int32_t k, const void* x, cons
     a.out = out;
     a.mode = epilogue;
     a.out_dtype = out_dtype;
-    return launched(launch_gemm_fp8(a, workspace, st), "linear launch");
+    return launched(launch_gemm_fp8(a, ws.plan, reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ws.partial),
+                                    st), "linear launch");
 }
 
 fvsr_status fvsr_layernorm_train(int64_t m, int32_t c, const void* x, int32_t dtype, const void* weight,

@@ -504,11 +504,12 @@ cudaError_t read_and_clear_device_error(int* flag, cudaStream_t st) {
         e = cudaMemcpyToSymbol(g_fvsr_timeout, &zero, sizeof(int));
         if (e != cudaSuccess) return e;
     }
-    int vp = 0, vs = 0, vg = 0;
+    int vp = 0, vs = 0, vg = 0, v8 = 0;
     e = read_and_clear_persist_error(&vp);
     if (e == cudaSuccess) e = read_and_clear_select_error(&vs);
     if (e == cudaSuccess) e = read_and_clear_gemm_error(&vg);
-    *flag = v | vp | vs | vg;
+    if (e == cudaSuccess) e = read_and_clear_gemm_fp8_error(&v8);
+    *flag = v | vp | vs | vg | v8;
     return e;
 }
 

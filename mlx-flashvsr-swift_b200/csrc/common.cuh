@@ -185,6 +185,8 @@ struct GemmArgs {
 cudaError_t launch_gemm_bf16(const GemmArgs& args, const void* A, const void* B, cudaStream_t st);
 size_t gemm_smem_bytes();
 cudaError_t read_and_clear_gemm_error(int* flag);
+// The same for the linear layers on 8-bit operands (gemm_fp8.cu; their launchers are in fp8.cuh).
+cudaError_t read_and_clear_gemm_fp8_error(int* flag);
 // Row normalisations of the DiT block (norm.cu); x / out (m, ch) bf16, ch a multiple of 256 up to 2048.
 cudaError_t launch_layernorm(int m, int ch, const void* x, const void* weight, const void* bias, const void* shift,
                              const void* scale, float eps, void* out, cudaStream_t st);

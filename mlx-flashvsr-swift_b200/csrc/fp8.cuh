@@ -81,7 +81,14 @@ struct Fp8GemmArgs {
     void* out;
     int mode, out_dtype;
 };
-cudaError_t launch_gemm_fp8(const Fp8GemmArgs& a, void* workspace, cudaStream_t st);
+// How a product is cut: `splits` parts of the sum over K, part_blocks blocks of 128 each (a multiple of 4: whole tiles of
+// codes) except the last; more than one part leaves fp32 partial products (splits, M, N) in the workspace.
+struct Fp8GemmPlan {
+    int splits, part_blocks;
+    size_t partial_bytes;
+};
+Fp8GemmPlan plan_gemm_fp8(int M, int N, int K);
+cudaError_t launch_gemm_fp8(const Fp8GemmArgs& a, const Fp8GemmPlan& plan, float* partial, cudaStream_t st);
 
 // LayerNorm for training (norm_train.cu).
 struct NormTrainArgs {

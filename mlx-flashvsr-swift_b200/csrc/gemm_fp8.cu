@@ -1,72 +1,408 @@
 // gemm_fp8.cu — the linear layers on 8-bit operands: out = epilogue(x · wᵀ + bias), x (M, K) and w (N, K) in the 8-bit
 // form of fp8.cuh (a scale for each block of 128 along K), fp32 sums, one rounding at the end.
+//
+//   out[m][n] = epi(Σ_b 2^(ex[m][b] + ew[n][b]) · Σ_{k in block b} x8[m][k]·w8[n][k] + bias[n])
+//
+// The scales are powers of two in the layout tensor memory wants, so the tensor core applies them itself
+// (tcgen05 kind::mxf8f6f4, one scale for 32 values along K): the four MMAs of a 128-wide block name the same byte of the
+// scale words, and one 512-byte copy to tensor memory serves 128 rows × 4 blocks. Nothing is promoted or rescaled in
+// registers, and a weight gradient (a scale for each row and block on both sides) costs what a forward product does.
+//
+// Persistent kernel over CTA pairs (clusters of two CTAs, one TPC): a pair walks 256 × 256 output tiles, CTA r of it
+// loading rows [m0 + 128r, +128) of x and [n0 + 128r, +128) of w per 128-wide K step (32 KB a stage, 6 stages) and, every
+// fourth step, the codes of its 128 rows of x and of all 256 rows of w. Warp roles (320 threads per CTA):
+//   warp 0      TMA producer;
+//   warp 1      TMEM owner and, in the even CTA, the issuer of the scale copies and MMAs (M 256, N 256, K 32);
+//   warps 2..9  epilogue: thread = output row = TMEM lane, each half of the warps 128 of the tile's columns.
+// Tensor memory (512 columns): accumulator 0 in [0, 256), accumulator 1 in [240, 496), the scales in [496, 508). The two
+// accumulators share 16 columns, which an epilogue reads first and releases (ovl) before anything else, so the next
+// tile's MMAs start some hundred cycles into the epilogue and run beside the rest of it.
+// When the tiles are fewer than the pairs, the sum over K is cut into parts (whole tiles of codes, 512 wide) that leave
+// fp32 partial products; a second kernel adds them in order and applies the epilogue.
+// Every wait is bounded (4 s); on expiry the kernel raises its abort and device timeout words, skips the rest of its
+// work and fvsr_device_check reports FVSR_ETIMEOUT.
 #include "../../include/fvsr_lcsa.h"
 #include "common.cuh"
 #include "fp8.cuh"
+#include "sm100.cuh"
 
 namespace fvsr {
 
+__device__ int g_gemm_fp8_timeout = 0;
+
 namespace {
 
-constexpr int kTM = 64, kTN = 64, kThreads = 256;
+using namespace sm100;
 
+constexpr int kBM = 256, kBN = 256, kBK = 128, kStages = 6;
+constexpr uint32_t kHalfBytes = 128 * kBK;       // 16 KB: one CTA's rows of x or of w per K step
+constexpr uint32_t kStageBytes = 2 * kHalfBytes;
+constexpr uint32_t kScaleBytes = 3 * 512;        // x's 128 rows, w's 256 rows, four blocks
+constexpr int kThreads = 320;
+constexpr int kEpiWarps = 8, kEpiThreads = 32 * kEpiWarps;
+constexpr uint64_t kWaitLimitNs = 4000000000ull;
+constexpr uint32_t kIdesc = idesc_mxf8(kBM, kBN);
+constexpr uint32_t kAcc1 = 240, kTmemScale = 496;
+constexpr int kBarFull = 0, kBarEmpty = kStages, kBarAccFull = 2 * kStages, kBarAccEmpty = 2 * kStages + 2,
+              kBarOvl = 2 * kStages + 4, kNumBars = 2 * kStages + 5;
+constexpr uint32_t kOffScale = kStages * kStageBytes;
+constexpr uint32_t kOffBar = kOffScale + kStages * kScaleBytes;
+constexpr uint32_t kOffTmemSlot = kOffBar + 8 * kNumBars;
+constexpr uint32_t kOffAbort = kOffTmemSlot + 4;
+constexpr uint32_t kOffCols = (kOffAbort + 4 + 15) & ~15u;  // bias[256], gate[256] as fp32
+constexpr uint32_t kSmemBytes = 1024 + kOffCols + 2 * kBN * 4;
+static_assert(kSmemBytes <= 232448, "shared memory");
+
+// GELU with the tanh approximation, 0.5·x·(1 + tanh(√(2/π)·(x + 0.044715·x³))) = x / (1 + 2^z), z = x·(c0 + c1·x²),
+// c0 = −2·√(2/π)·log2(e), c1 = 0.044715·c0; 2^z overflowing gives −0, underflowing gives x.
 __device__ __forceinline__ float gelu_tanh(float x) {
-    return 0.5f * x * (1.0f + tanhf(0.7978845608028654f * (x + 0.044715f * x * x * x)));
+    constexpr float c0 = -2.0f * 0.7978845608028654f * 1.4426950408889634f, c1 = 0.044715f * c0;
+    return x * rcp_approx(1.0f + ex2_approx(x * fmaf(c1, x * x, c0)));
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) gemm_fp8_simple_kernel(const Fp8GemmArgs a) {
-    __shared__ float xs[kTM][33], ws[kTN][33];
-    griddep_wait_then_release();
-    const int m0 = blockIdx.y * kTM, n0 = blockIdx.x * kTN;
-    const int64_t ld = fp8_ld(a.K), tiles = fp8_scale_tiles(a.K);
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    float acc[4][4] = {};
-    for (int k0 = 0; k0 < (int)ld; k0 += 32) {
-        for (int i = threadIdx.x; i < 64 * 16; i += kThreads) {
-            const int r = i / 16, c = (i % 16) * 2;
-            float lo = 0.0f, hi = 0.0f;
-            if (m0 + r < a.M) {
-                fp8_unpack2(*reinterpret_cast<const uint16_t*>(a.x + (m0 + r) * ld + k0 + c), lo, hi);
-                const float s = fp8_down(a.x_scale[fp8_code_pos(m0 + r, k0 >> 7, tiles)]);
-                lo *= s, hi *= s;
+__device__ __forceinline__ float finish(float acc, float bias, float gate, const T* resid, int mode) {
+    float y = acc + bias;
+    if (mode == FVSR_LINEAR_GELU) y = gelu_tanh(y);
+    if (mode == FVSR_LINEAR_GATED_RESIDUAL) y = fmaf(gate, y, load_as_float(resid));
+    return y;
+}
+
+// 32 consecutive output columns of one row. n = how many of them exist; vec: the row's columns are 16-byte aligned and
+// all there.
+template <typename T, int kMode>
+__device__ __forceinline__ void epilogue_chunk(const uint32_t* v, const float* bias, const float* gate, const T* resid,
+                                               T* out, int n, bool vec) {
+    if (vec) {
+#pragma unroll
+        for (int i = 0; i < 32; i += 8) {
+            float r[8], y[8];
+            if (kMode == FVSR_LINEAR_GATED_RESIDUAL) {
+                if (sizeof(T) == 2) {
+                    const uint4 u = *reinterpret_cast<const uint4*>(resid + i);
+                    bf2_to_f(u.x, r[0], r[1]), bf2_to_f(u.y, r[2], r[3]);
+                    bf2_to_f(u.z, r[4], r[5]), bf2_to_f(u.w, r[6], r[7]);
+                } else {
+                    *reinterpret_cast<float4*>(r) = *reinterpret_cast<const float4*>(resid + i);
+                    *reinterpret_cast<float4*>(r + 4) = *reinterpret_cast<const float4*>(resid + i + 4);
+                }
             }
-            xs[r][c] = lo, xs[r][c + 1] = hi;
-            lo = hi = 0.0f;
-            if (n0 + r < a.N) {
-                fp8_unpack2(*reinterpret_cast<const uint16_t*>(a.w + (n0 + r) * ld + k0 + c), lo, hi);
-                const float s = fp8_down(a.w_scale[fp8_code_pos(n0 + r, k0 >> 7, tiles)]);
-                lo *= s, hi *= s;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                y[j] = __uint_as_float(v[i + j]) + bias[i + j];
+                if (kMode == FVSR_LINEAR_GELU) y[j] = gelu_tanh(y[j]);
+                if (kMode == FVSR_LINEAR_GATED_RESIDUAL) y[j] = fmaf(gate[i + j], y[j], r[j]);
             }
-            ws[r][c] = lo, ws[r][c + 1] = hi;
+            if (sizeof(T) == 2) {
+                *reinterpret_cast<uint4*>(out + i) = make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]),
+                                                                pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7]));
+            } else {
+                *reinterpret_cast<float4*>(out + i) = make_float4(y[0], y[1], y[2], y[3]);
+                *reinterpret_cast<float4*>(out + i + 4) = make_float4(y[4], y[5], y[6], y[7]);
+            }
         }
-        __syncthreads();
+    } else {
 #pragma unroll
-        for (int k = 0; k < 32; ++k)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(xs[ty * 4 + i][k], ws[tx + 16 * j][k], acc[i][j]);
-        __syncthreads();
+        for (int i = 0; i < 32; ++i)
+            if (i < n) store_from_float(out + i, finish(__uint_as_float(v[i]), bias[i], gate[i], resid + i, kMode));
     }
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const int64_t m = m0 + ty * 4 + i, n = n0 + tx + 16 * j;
-            if (m >= a.M || n >= a.N) continue;
-            float y = acc[i][j] + (a.bias ? __bfloat162float(a.bias[n]) : 0.0f);
-            if (a.mode == FVSR_LINEAR_GELU) y = gelu_tanh(y);
-            if (a.mode == FVSR_LINEAR_GATED_RESIDUAL)
-                y = fmaf(__bfloat162float(a.gate[n]), y, load_as_float(static_cast<const T*>(a.resid) + m * a.N + n));
-            store_from_float(static_cast<T*>(a.out) + m * a.N + n, y);
+}
+
+struct Work {
+    int mt, nt, kt, splits, part_blocks;
+};
+
+template <typename T, int kMode>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    gemm_fp8_sm100_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
+                          const __grid_constant__ CUtensorMap tmXS, const __grid_constant__ CUtensorMap tmWS,
+                          const Fp8GemmArgs a, const Work wk) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const uint32_t sbase = smem_u32(smem);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const int pair = (int)(blockIdx.x >> 1), npairs = (int)(gridDim.x >> 1);
+    const int items = wk.mt * wk.nt * wk.splits;
+    volatile uint32_t* abort_word = reinterpret_cast<volatile uint32_t*>(smem + kOffAbort);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kOffTmemSlot);
+    auto bar = [&](int i) { return sbase + kOffBar + 8u * (uint32_t)i; };
+    auto wait = [&](int b, uint32_t parity) {
+        return mbar_wait(bar(b), parity & 1u, abort_word, &g_gemm_fp8_timeout, kWaitLimitNs);
+    };
+    // item → output tile (columns fastest) and blocks [kb0, kb1) of K
+    auto place = [&](int t, int& m0, int& n0, int& kb0, int& kb1) {
+        const int tile = t / wk.splits, part = t % wk.splits;
+        m0 = tile / wk.nt * kBM, n0 = tile % wk.nt * kBN;
+        kb0 = part * wk.part_blocks, kb1 = min(kb0 + wk.part_blocks, wk.kt);
+    };
+    if (threadIdx.x == 0) {
+        for (int st = 0; st < kStages; ++st) {
+            mbar_init(bar(kBarFull + st), 1);
+            mbar_init(bar(kBarEmpty + st), 1);
         }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(bar(kBarAccFull + b), 1);
+            mbar_init(bar(kBarAccEmpty + b), 2 * kEpiWarps);
+        }
+        mbar_init(bar(kBarOvl), kEpiWarps);
+        *abort_word = 0;
+        fence_mbar_init();
+    }
+    if (warp == 0 && lane == 0) {
+        prefetch_tmap(&tmX);
+        prefetch_tmap(&tmW);
+        prefetch_tmap(&tmXS);
+        prefetch_tmap(&tmWS);
+    }
+    griddep_wait_then_release();
+    if (warp == 1) {
+        tmem_alloc_pair(smem_u32(tmem_slot), 512);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before();
+    cluster_sync();  // both CTAs' barriers are initialised and their TMEM allocated before any remote signal
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 0) {
+        // ---------------- TMA producer: rows past the tensors' ends read as zeros with scale code 0 ----------------
+        if (lane == 0) {
+            uint32_t it = 0;
+            bool ok = true;
+            for (int t = pair; ok && t < items; t += npairs) {
+                int m0, n0, kb0, kb1;
+                place(t, m0, n0, kb0, kb1);
+                m0 += 128 * (int)rank;
+                const int nr = n0 + 128 * (int)rank;
+                for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                    const int st = (int)(it % kStages);
+                    if (it >= kStages && !(ok = wait(kBarEmpty + st, it / kStages - 1))) break;
+                    const uint32_t dst = sbase + (uint32_t)st * kStageBytes;
+                    const uint32_t sdst = sbase + kOffScale + (uint32_t)st * kScaleBytes;
+                    const uint32_t full0 = mapa_shared(bar(kBarFull + st), 0);
+                    const bool scales = (kb & 3) == 0;
+                    if (rank == 0) mbar_expect_tx(bar(kBarFull + st), 2 * (kStageBytes + (scales ? kScaleBytes : 0)));
+                    tma_load_2d_pair(dst, &tmX, kb * kBK, m0, full0);
+                    tma_load_2d_pair(dst + kHalfBytes, &tmW, kb * kBK, nr, full0);
+                    if (scales) {
+                        const int g = kb >> 2, kt4 = (wk.kt + 3) >> 2;
+                        tma_load_2d_pair(sdst, &tmXS, 0, (m0 >> 7) * kt4 + g, full0);
+                        tma_load_2d_pair(sdst + 512, &tmWS, 0, (n0 >> 7) * kt4 + g, full0);
+                        tma_load_2d_pair(sdst + 1024, &tmWS, 0, ((n0 >> 7) + 1) * kt4 + g, full0);
+                    }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // ---------------- MMA issuer: one thread of the even CTA ----------------
+        if (lane == 0 && rank == 0) {
+            uint32_t it = 0;
+            bool ok = true;
+            int lt = 0;
+            for (int t = pair; ok && t < items; t += npairs, ++lt) {
+                int m0, n0, kb0, kb1;
+                place(t, m0, n0, kb0, kb1);
+                const int acc = lt & 1;
+                if (lt >= 2 && !(ok = wait(kBarAccEmpty + acc, (uint32_t)((lt >> 1) - 1)))) break;
+                if (lt >= 1 && !(ok = wait(kBarOvl, (uint32_t)(lt - 1)))) break;
+                tc_fence_after();
+                const uint32_t d = tmem + (acc ? kAcc1 : 0u), sf = tmem + kTmemScale;
+                for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                    const int st = (int)(it % kStages);
+                    if (!(ok = wait(kBarFull + st, it / kStages))) break;
+                    tc_fence_after();
+                    const uint32_t sa = sbase + (uint32_t)st * kStageBytes;
+                    if ((kb & 3) == 0) {
+                        const uint32_t sc = sbase + kOffScale + (uint32_t)st * kScaleBytes;
+                        tmem_cp_scales_pair(sf, scale_desc(sc));
+                        tmem_cp_scales_pair(sf + 4, scale_desc(sc + 512));
+                        tmem_cp_scales_pair(sf + 8, scale_desc(sc + 1024));
+                    }
+                    const uint64_t ad = smem_desc(sa, 16, 1024);
+                    const uint64_t bd = smem_desc(sa + kHalfBytes, 16, 1024);
+                    const uint32_t idesc = kIdesc | idesc_sf_id((uint32_t)kb & 3u);
+#pragma unroll
+                    for (int kk = 0; kk < kBK / 32; ++kk)
+                        mma_mxf8_pair(d, ad + (uint64_t)(2 * kk), bd + (uint64_t)(2 * kk), idesc, sf, sf + 4,
+                                      (kb > kb0 || kk > 0) ? 1u : 0u);
+                    mma_commit_pair(bar(kBarEmpty + st));
+                    mma_commit_pair(mapa_shared(bar(kBarEmpty + st), 1));
+                }
+                if (ok) {
+                    mma_commit_pair(bar(kBarAccFull + acc));
+                    mma_commit_pair(mapa_shared(bar(kBarAccFull + acc), 1));
+                }
+            }
+        }
+    } else {
+        // ---------------- epilogue: this CTA's 128 rows; thread = row = TMEM lane, half = which 128 columns ----------------
+        const int quarter = warp & 3, half = (warp - 2) >> 2;
+        const int r = quarter * 32 + lane;
+        const int et = threadIdx.x - 64;
+        const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * (kBN / 2));
+        float* bias_s = reinterpret_cast<float*>(smem + kOffCols);
+        float* gate_s = bias_s + kBN;
+        const uint32_t acc_empty0 = mapa_shared(bar(kBarAccEmpty), 0), ovl0 = mapa_shared(bar(kBarOvl), 0);
+        const bool aligned_rows = ((int64_t)a.N * sizeof(T)) % 16 == 0 &&
+                                  ((reinterpret_cast<uintptr_t>(a.out) | reinterpret_cast<uintptr_t>(a.resid)) & 15) == 0;
+        int lt = 0;
+        bool ok = true;
+        for (int t = pair; t < items; t += npairs, ++lt) {
+            int m0, n0, kb0, kb1;
+            place(t, m0, n0, kb0, kb1);
+            const int acc = lt & 1;
+            named_barrier_sync(1, kEpiThreads);
+            bias_s[et] = a.bias && n0 + et < a.N ? __bfloat162float(a.bias[n0 + et]) : 0.0f;
+            gate_s[et] = kMode == FVSR_LINEAR_GATED_RESIDUAL && n0 + et < a.N ? __bfloat162float(a.gate[n0 + et]) : 0.0f;
+            named_barrier_sync(1, kEpiThreads);
+            const int64_t row = (int64_t)m0 + 128 * (int)rank + r;
+            const int c0 = n0 + half * (kBN / 2);
+            const int64_t at = (wk.splits > 1 ? (int64_t)(t % wk.splits) * a.M * a.N : 0) + row * a.N + c0;
+            if (ok) ok = __all_sync(0xffffffffu, wait(kBarAccFull + acc, (uint32_t)(lt >> 1)));
+            if (!ok) continue;
+            tc_fence_after();
+            T* orow = static_cast<T*>(a.out) + at;
+            const T* rrow = static_cast<const T*>(a.resid) + at;
+            const float *bcol = bias_s + half * (kBN / 2), *gcol = gate_s + half * (kBN / 2);
+            const uint32_t tbase = lane_base + (acc ? kAcc1 : 0u);
+            // accumulator 0 from its last chunk to its first, accumulator 1 from its first: the shared columns come first
+            auto chunk = [&](int i) { return acc ? i : kBN / 64 - 1 - i; };
+            auto emit = [&](const uint32_t* v, int c) {
+                const int left = a.N - (c0 + 32 * c);
+                if (row < a.M && left > 0)
+                    epilogue_chunk<T, kMode>(v, bcol + 32 * c, gcol + 32 * c, rrow + 32 * c, orow + 32 * c, left,
+                                             aligned_rows && left >= 32);
+            };
+            uint32_t va[32], vb[32];
+            tmem_ld32(tbase + 32u * (uint32_t)chunk(0), va);
+            tmem_ld_wait(va);
+            if (half != acc) {  // this half held the shared columns: half 1 of accumulator 0, half 0 of accumulator 1
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(ovl0);
+            }
+#pragma unroll
+            for (int i = 0; i < kBN / 64; i += 2) {
+                tmem_ld32(tbase + 32u * (uint32_t)chunk(i + 1), vb);
+                emit(va, chunk(i));
+                tmem_ld_wait(vb);
+                if (i + 2 < kBN / 64) tmem_ld32(tbase + 32u * (uint32_t)chunk(i + 2), va);
+                emit(vb, chunk(i + 1));
+                if (i + 2 < kBN / 64) tmem_ld_wait(va);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(acc_empty0 + 8u * (uint32_t)acc);
+        }
+    }
+    tc_fence_before();
+    cluster_sync();  // no signal to the other CTA and no MMA on this CTA's shared memory is still in flight
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem, 512);
+    }
+}
+
+// out = epilogue(Σ partial products in order + bias), one thread per element.
+template <typename T>
+__global__ void __launch_bounds__(256) gemm_fp8_join_kernel(const Fp8GemmArgs a, const float* __restrict__ partial,
+                                                            int splits) {
+    griddep_wait_then_release();
+    const int64_t n = (int64_t)a.M * a.N;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        float s = partial[i];
+        for (int p = 1; p < splits; ++p) s += partial[p * n + i];
+        const int c = (int)(i % a.N);
+        store_from_float(static_cast<T*>(a.out) + i,
+                         finish(s, a.bias ? __bfloat162float(a.bias[c]) : 0.0f,
+                                a.gate ? __bfloat162float(a.gate[c]) : 0.0f, static_cast<const T*>(a.resid) + i, a.mode));
+    }
+}
+
+int sm_count() {
+    int dev = 0, n = 148;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+        n = 148;
+    return n;
+}
+
+template <typename T, int kMode>
+cudaError_t launch_tiles(const Fp8GemmArgs& args, const Work& wk, const CUtensorMap (&maps)[4], cudaStream_t st) {
+    auto kernel = gemm_fp8_sm100_kernel<T, kMode>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes);
+    if (e != cudaSuccess) return e;
+    const int items = wk.mt * wk.nt * wk.splits, pairs = sm_count() / 2;
+    return launch_pdl(kernel, dim3(2 * (items < pairs ? items : pairs)), dim3(kThreads), kSmemBytes, st, maps[0],
+                      maps[1], maps[2], maps[3], args, wk);
+}
+
+template <typename T>
+cudaError_t launch_mode(const Fp8GemmArgs& args, const Work& wk, const CUtensorMap (&maps)[4], cudaStream_t st) {
+    switch (args.mode) {
+        case FVSR_LINEAR: return launch_tiles<T, FVSR_LINEAR>(args, wk, maps, st);
+        case FVSR_LINEAR_GELU: return launch_tiles<T, FVSR_LINEAR_GELU>(args, wk, maps, st);
+        default: return launch_tiles<T, FVSR_LINEAR_GATED_RESIDUAL>(args, wk, maps, st);
+    }
 }
 
 }  // namespace
 
-cudaError_t launch_gemm_fp8(const Fp8GemmArgs& a, void*, cudaStream_t st) {
-    const dim3 grid((a.N + kTN - 1) / kTN, (a.M + kTM - 1) / kTM);
-    return a.out_dtype == FVSR_BF16 ? launch_pdl(gemm_fp8_simple_kernel<__nv_bfloat16>, grid, dim3(kThreads), 0, st, a)
-                                    : launch_pdl(gemm_fp8_simple_kernel<float>, grid, dim3(kThreads), 0, st, a);
+Fp8GemmPlan plan_gemm_fp8(int M, int N, int K) {
+    Fp8GemmPlan p{1, 0, 0};
+    const int kt = (K + kBK - 1) / kBK, groups = (kt + 3) / 4;
+    const int64_t tiles = (int64_t)((M + kBM - 1) / kBM) * ((N + kBN - 1) / kBN);
+    const int pairs = sm_count() / 2;
+    int splits = tiles * 2 <= pairs ? (int)(pairs / tiles) : 1;
+    if (splits > groups) splits = groups;
+    const int per = (groups + splits - 1) / splits;
+    p.splits = (groups + per - 1) / per;
+    p.part_blocks = 4 * per;
+    if (p.splits > 1) p.partial_bytes = (size_t)p.splits * M * N * sizeof(float);
+    return p;
+}
+
+cudaError_t launch_gemm_fp8(const Fp8GemmArgs& args, const Fp8GemmPlan& plan, float* partial, cudaStream_t st) {
+    Work wk;
+    wk.mt = (args.M + kBM - 1) / kBM;
+    wk.nt = (args.N + kBN - 1) / kBN;
+    wk.kt = (args.K + kBK - 1) / kBK;
+    wk.splits = plan.splits;
+    wk.part_blocks = plan.part_blocks;
+    CUtensorMap maps[4];
+    const int64_t ld = fp8_ld(args.K), kt4 = fp8_scale_tiles(args.K);
+    if (!make_byte_map(&maps[0], args.x, args.M, ld, 128) || !make_byte_map(&maps[1], args.w, args.N, ld, 128) ||
+        !make_scale_map(&maps[2], args.x_scale, ((int64_t)args.M + 127) / 128 * kt4) ||
+        !make_scale_map(&maps[3], args.w_scale, ((int64_t)args.N + 127) / 128 * kt4))
+        return cudaErrorInvalidValue;
+    if (plan.splits == 1)
+        return args.out_dtype == FVSR_BF16 ? launch_mode<__nv_bfloat16>(args, wk, maps, st)
+                                           : launch_mode<float>(args, wk, maps, st);
+    Fp8GemmArgs parts = args;
+    parts.out = partial;
+    parts.bias = nullptr;
+    parts.mode = FVSR_LINEAR;
+    parts.resid = nullptr;
+    cudaError_t e = launch_tiles<float, FVSR_LINEAR>(parts, wk, maps, st);
+    if (e != cudaSuccess) return e;
+    const int64_t blocks = ((int64_t)args.M * args.N + 255) / 256, most = (int64_t)sm_count() * 8;
+    const dim3 grid((unsigned)(blocks < most ? blocks : most));
+    return args.out_dtype == FVSR_BF16
+               ? launch_pdl(gemm_fp8_join_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, args, (const float*)partial,
+                            plan.splits)
+               : launch_pdl(gemm_fp8_join_kernel<float>, grid, dim3(256), 0, st, args, (const float*)partial, plan.splits);
+}
+
+cudaError_t read_and_clear_gemm_fp8_error(int* flag) {
+    int v = 0;
+    cudaError_t e = cudaMemcpyFromSymbol(&v, g_gemm_fp8_timeout, sizeof(int));
+    if (e != cudaSuccess) return e;
+    if (v) {
+        const int zero = 0;
+        e = cudaMemcpyToSymbol(g_gemm_fp8_timeout, &zero, sizeof(int));
+    }
+    *flag = v;
+    return e;
 }
 
 }  // namespace fvsr

@@ -201,6 +201,21 @@ __device__ __forceinline__ void mma_ss_pair(uint32_t d_tmem, uint64_t adesc, uin
         "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+// The same on e4m3 operands with an e8m0 scale for each row and 32 values along K (kind::mxf8f6f4, K 32): the scales'
+// codes are in tensor memory, row r of a 128-row group in lane r % 32 (of every quarter), byte sf_id of column r / 32.
+__device__ __forceinline__ void mma_mxf8_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                              uint32_t sfa_tmem, uint32_t sfb_tmem, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(sfa_tmem), "r"(sfb_tmem)
+        : "memory");
+}
+// Copies 512 bytes (32 lanes × 16 bytes) of each CTA's shared memory to four columns of its tensor memory, repeated in
+// every quarter of the lanes. In order with the MMAs that the same thread issues after it.
+__device__ __forceinline__ void tmem_cp_scales_pair(uint32_t taddr, uint64_t sdesc) {
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
+}
 // Arrive once on the mbarrier at `bar_cluster` (either CTA) when this thread's pair MMAs so far have completed.
 __device__ __forceinline__ void mma_commit_pair(uint32_t bar_cluster) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar_cluster)
@@ -212,6 +227,17 @@ __device__ __forceinline__ void mma_commit_pair(uint32_t bar_cluster) {
 __host__ __device__ constexpr uint32_t idesc_bf16_f32(int m, int n, int a_mn_major, int b_mn_major) {
     return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)a_mn_major << 15) | ((uint32_t)b_mn_major << 16) |
            ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+
+// Instruction descriptor of kind::mxf8f6f4 with e4m3 operands, both K-major: scale format e8m0 at bit 23, N >> 3 at bits
+// 17-22, M >> 4 at bits 24-28; idesc_sf_id adds the byte of the scale words that A (bits 29-30) and B (4-5) use.
+__host__ __device__ constexpr uint32_t idesc_mxf8(int m, int n) {
+    return (1u << 23) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+__host__ __device__ constexpr uint32_t idesc_sf_id(uint32_t id) { return (id << 29) | (id << 4); }
+// Descriptor of 512 bytes of scale codes (no swizzle; 8-row groups of 16-byte rows, 128 bytes apart).
+__device__ __forceinline__ uint64_t scale_desc(uint32_t saddr) {
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
 }
 
 // Shared-memory matrix descriptor (sm_100 version 1): start >> 4 at bits 0-13, leading byte offset >> 4 at 16-29,
@@ -321,6 +347,32 @@ inline bool make_tile_map_box(CUtensorMap* map, const void* base, int64_t rows, 
     const cuuint32_t estr[2] = {1, 1};
     return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// 2-D map over (rows, row_bytes) bytes, a box of box_rows rows × 128 bytes, 128-byte swizzle: the 8-bit operand tiles.
+inline bool make_byte_map(CUtensorMap* map, const void* base, int64_t rows, int64_t row_bytes, int box_rows) {
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (!fn || box_rows < 1 || box_rows > 256) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)row_bytes, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)row_bytes};
+    const cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// 2-D map over tiles of 512 bytes (128 words), one tile a box, as stored.
+inline bool make_scale_map(CUtensorMap* map, const void* base, int64_t tiles) {
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (!fn) return false;
+    const cuuint64_t dims[2] = {128, (cuuint64_t)tiles};
+    const cuuint64_t strides[1] = {512};
+    const cuuint32_t box[2] = {128, 1};
+    const cuuint32_t estr[2] = {1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(base), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
