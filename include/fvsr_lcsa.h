@@ -348,6 +348,7 @@ fvsr_status fvsr_cross_attention(int32_t heads, int32_t lq, int32_t lk, const vo
  * e4m3's normal range). A block that holds an infinity or a NaN has code 255 and reads back as NaN throughout.
  *
  * fvsr_fp8_bytes — the two sizes for (rows, cols); either pointer may be NULL.
+ * fvsr_fp8_codes — the codes in order, out (rows, ceil(cols / 128)) bytes.
  * fvsr_quantize_fp8 — x (rows, cols), dtype FVSR_BF16 or FVSR_F32, into its form (q, scale) and / or the form of its
  * transpose, a (cols, rows) tensor (qt, scale_t); a pair may be NULL, not both. square = 0: one scale for each row's
  * block (of x for q, of its transpose for qt); 1: one for each 128 x 128 square of x, the same for both forms (weights).
@@ -355,6 +356,7 @@ fvsr_status fvsr_cross_attention(int32_t heads, int32_t lq, int32_t lk, const vo
  * rows >= 0, 1 <= cols, rows and cols at most 2^30, rows * cols at most 2^40. 16-byte alignment for x, q, qt and the
  * scales; 4-byte for the tensor read back into. */
 fvsr_status fvsr_fp8_bytes(int64_t rows, int64_t cols, size_t* value_bytes, size_t* scale_bytes);
+fvsr_status fvsr_fp8_codes(int64_t rows, int64_t cols, const void* scale, void* out, fvsr_stream_t stream);
 fvsr_status fvsr_quantize_fp8(int64_t rows, int64_t cols, const void* x, int32_t dtype, int32_t square, void* q,
                               void* scale, void* qt, void* scale_t, fvsr_stream_t stream);
 fvsr_status fvsr_dequantize_fp8(int64_t rows, int64_t cols, const void* q, const void* scale, void* out, int32_t dtype,

@@ -40,7 +40,7 @@ EXPORTED = [
     "fvsr_stream_workspace_size", "fvsr_stream_start_chunk", "fvsr_stream_rope", "fvsr_stream_layer",
     "fvsr_kv_cache_create_padded", "fvsr_kv_cache_reserve", "fvsr_kv_cache_commit", "fvsr_lcsa_forward_shard",
     "fvsr_lcsa_partial_size", "fvsr_lcsa_select_shard", "fvsr_lcsa_attend_shard", "fvsr_linear", "fvsr_linear_qkv",
-    "fvsr_layernorm", "fvsr_rmsnorm", "fvsr_cross_attention", "fvsr_fp8_bytes", "fvsr_quantize_fp8",
+    "fvsr_layernorm", "fvsr_rmsnorm", "fvsr_cross_attention", "fvsr_fp8_bytes", "fvsr_fp8_codes", "fvsr_quantize_fp8",
     "fvsr_dequantize_fp8", "fvsr_linear_fp8_workspace_size", "fvsr_linear_fp8", "fvsr_layernorm_train",
     "fvsr_layernorm_backward_workspace_size", "fvsr_layernorm_backward",
 ]
@@ -133,6 +133,7 @@ def lib() -> ctypes.CDLL:
         "fvsr_rmsnorm": ([I32, I32, P, P, ctypes.c_float, P, P], ctypes.c_int),
         "fvsr_cross_attention": ([I32, I32, I32, P, P, P, P, P], ctypes.c_int),
         "fvsr_fp8_bytes": ([I64, I64, ctypes.POINTER(SZ), ctypes.POINTER(SZ)], ctypes.c_int),
+        "fvsr_fp8_codes": ([I64, I64, P, P, P], ctypes.c_int),
         "fvsr_quantize_fp8": ([I64, I64, P, I32, I32, P, P, P, P, P], ctypes.c_int),
         "fvsr_dequantize_fp8": ([I64, I64, P, P, P, I32, P], ctypes.c_int),
         "fvsr_linear_fp8_workspace_size": ([I32, I32, I32, I32, ctypes.POINTER(SZ)], ctypes.c_int),
@@ -734,6 +735,16 @@ class Fp8Tensor:
             raise FVSRError(FVSR_EINVAL, "the parts of an 8-bit tensor must be contiguous on one CUDA device")
         self.data, self.scale, self.rows, self.cols = data, scale, int(rows), int(cols)
 
+    @staticmethod
+    def empty_like(x, rows: int, cols: int) -> "Fp8Tensor":
+        """Room for a (rows, cols) tensor in 8 bits on x's device, its contents undefined."""
+        torch = _torch()
+        t = Fp8Tensor.__new__(Fp8Tensor)
+        t.data = x.new_empty((rows, (cols + 127) // 128 * 128), dtype=torch.float8_e4m3fn)
+        t.scale = x.new_empty(((rows + 127) // 128, (cols + 511) // 512, 512), dtype=torch.uint8)
+        t.rows, t.cols = rows, cols
+        return t
+
     @property
     def device(self):
         return self.data.device
@@ -742,66 +753,84 @@ class Fp8Tensor:
     def shape(self):
         return (self.rows, self.cols)
 
-    def codes(self):
-        """The blocks' codes (rows, ceil(cols / 128)) uint8, a view: a block's scale is 2^(code - 127)."""
-        rt, kt, _ = self.scale.shape
-        full = self.scale.view(rt, kt, 32, 4, 4).permute(0, 3, 2, 1, 4).reshape(rt * 128, kt * 4)
-        return full[:self.rows, :(self.cols + 127) // 128]
-
-    @staticmethod
-    def empty(rows: int, cols: int, device="cuda") -> "Fp8Tensor":
-        torch = _torch()
-        return Fp8Tensor(
-            torch.empty((rows, (cols + 127) // 128 * 128), dtype=torch.float8_e4m3fn, device=device),
-            torch.empty(((rows + 127) // 128, (cols + 511) // 512, 512), dtype=torch.uint8, device=device), rows, cols)
+    def codes(self, stream=None):
+        """The blocks' codes in order (fvsr_fp8_codes), (rows, ceil(cols / 128)) uint8: a block's scale is
+        2^(code - 127)."""
+        away = _elsewhere(self.scale, stream)
+        if away is not None:
+            with away:
+                return self.codes()
+        out = self.scale.new_empty((self.rows, (self.cols + 127) // 128))
+        _check(lib().fvsr_fp8_codes(self.rows, self.cols, self.scale.data_ptr(), out.data_ptr(), _here(out)))
+        return out
 
 
-class _Launch:
-    """`with _Launch(device, stream) as handle`: the device of the operands is current and the stream the launches go to
-    is the current one, so memory allocated inside belongs to that stream; handle is the stream's."""
-
-    __slots__ = ("device", "stream", "ctx")
-
-    def __init__(self, device, stream):
-        self.device, self.stream, self.ctx = device, stream, None
-
-    def __enter__(self):
-        torch = _torch()
-        if self.stream is not None:
-            if self.stream.device != self.device:
-                raise FVSRError(FVSR_EINVAL, f"the stream is on {self.stream.device}, the tensors on {self.device}")
-            self.ctx = torch.cuda.stream(self.stream)
-            self.ctx.__enter__()
-            return ctypes.c_void_p(self.stream.cuda_stream)
-        if torch.cuda.current_device() != self.device.index:
-            self.ctx = torch.cuda.device(self.device)
-            self.ctx.__enter__()
-        return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
-
-    def __exit__(self, *exc):
-        if self.ctx is not None:
-            self.ctx.__exit__(*exc)
-        return False
+def _elsewhere(t, stream):
+    """None when the current stream of the current device, t's, is where a call's launches and allocations belong; else
+    the context in which it is: memory allocated there belongs to the given stream."""
+    torch = _torch()
+    if stream is not None:
+        if stream.device != t.device:
+            raise FVSRError(FVSR_EINVAL, f"the stream is on {stream.device}, the tensors on {t.device}")
+        return torch.cuda.stream(stream)
+    if torch.cuda.current_device() != t.get_device():
+        return torch.cuda.device(t.get_device())
+    return None
 
 
-def _matrix(t, name, dtypes=None, shape=None, device=None):
+def _here(t) -> int:
+    """The handle of the current stream on t's device."""
+    return _torch()._C._cuda_getCurrentRawStream(t.get_device())
+
+
+def _matrix(t, name, dtypes=None, shape=None, like=None):
     """t as a contiguous 2-D CUDA tensor ((1, L, C) becomes (L, C)) of one of the dtypes, or FVSRError."""
     torch = _torch()
     if t.dim() == 3 and t.shape[0] == 1:
         t = t[0]
-    if t.dim() != 2 or t.dtype not in (dtypes or (torch.bfloat16, torch.float32)) or not t.is_cuda or \
-            not t.is_contiguous():
+    if t.dim() != 2 or not t.is_cuda or not t.is_contiguous() or \
+            t.dtype not in (dtypes or (torch.bfloat16, torch.float32)):
         raise FVSRError(FVSR_EINVAL, f"{name} must be a contiguous 2-D CUDA tensor, bfloat16 or float32 as the call allows")
-    if (shape is not None and tuple(t.shape) != shape) or (device is not None and t.device != device):
-        raise FVSRError(FVSR_EINVAL, f"{name} must be {shape} on {device}, got {tuple(t.shape)} on {t.device}")
+    if (shape is not None and t.shape != shape) or (like is not None and t.get_device() != like.get_device()):
+        raise FVSRError(FVSR_EINVAL, f"{name} must be {tuple(shape or t.shape)} beside the other tensors, got "
+                                     f"{tuple(t.shape)} on {t.device}")
     return t
 
 
-def _channel_vector(t, name, n, dtype, device):
-    if t is not None and (t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or t.device != device or
-                          not t.is_contiguous()):
-        raise FVSRError(FVSR_EINVAL, f"{name} must be contiguous ({n},) {dtype} on {device}")
-    return t
+def _channel_vector(t, name, n, dtype, like):
+    """The address of a contiguous (n,) tensor of dtype on like's device (None: no such vector), or FVSRError."""
+    if t is None:
+        return None
+    if t.dtype != dtype or t.shape != (n,) or t.get_device() != like.get_device() or not t.is_contiguous():
+        raise FVSRError(FVSR_EINVAL, f"{name} must be contiguous ({n},) {dtype} on {like.device}")
+    return t.data_ptr()
+
+
+def _bytes(fn, device: int, *args) -> int:
+    """A workspace size of the C ABI on the current device, remembered by its arguments."""
+    key = (fn, device, args)
+    size = _sizes.get(key)
+    if size is None:
+        n = ctypes.c_size_t(0)
+        _check(getattr(lib(), fn)(*args, ctypes.byref(n)))
+        if len(_sizes) > 4096:
+            _sizes.clear()
+        size = _sizes[key] = n.value
+    return size
+
+
+_sizes: dict = {}
+
+
+def _scratch(workspace, need: int, like):
+    """(address, bytes) of a workspace of at least `need` bytes: the given one or a new one, also returned to be held."""
+    if workspace is None:
+        if not need:
+            return None, 0, None
+        workspace = like.new_empty((need,), dtype=_torch().uint8)
+    elif workspace.get_device() != like.get_device() or not workspace.is_contiguous():
+        raise FVSRError(FVSR_EINVAL, f"the workspace must be contiguous on {like.device}")
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
 
 
 def quantize_fp8(x, square: bool = False, transpose: bool = False, out=None, stream=None) -> Fp8Tensor:
@@ -809,42 +838,53 @@ def quantize_fp8(x, square: bool = False, transpose: bool = False, out=None, str
     128, or with square for each 128 x 128 square (weights). transpose: the form of x's transpose, (cols, rows), whose
     blocks run along x's rows (the checkpoint a weight gradient reads)."""
     x = _matrix(x, "x")
+    away = _elsewhere(x, stream)
+    if away is not None:
+        with away:
+            return quantize_fp8(x, square, transpose, out)
     rows, cols = x.shape
-    with _Launch(x.device, stream) as st:
-        shape = (cols, rows) if transpose else (rows, cols)
-        if out is None:
-            out = Fp8Tensor.empty(*shape, device=x.device)
-        elif out.shape != shape or out.device != x.device:
-            raise FVSRError(FVSR_EINVAL, f"out must be an 8-bit tensor of {shape} on {x.device}")
-        held = (_ptr(out.data), _ptr(out.scale))
-        _check(lib().fvsr_quantize_fp8(rows, cols, _ptr(x), _dtype_code(x), int(bool(square)),
-                                       *((None, None) + held if transpose else held + (None, None)), st))
+    shape = (cols, rows) if transpose else (rows, cols)
+    if shape[1] == 0:
+        raise FVSRError(FVSR_EINVAL, f"a tensor of {shape} has no 8-bit form")
+    if out is None:
+        out = Fp8Tensor.empty_like(x, *shape)
+    elif out.shape != shape or out.device != x.device:
+        raise FVSRError(FVSR_EINVAL, f"out must be an 8-bit tensor of {shape} on {x.device}")
+    held = (out.data.data_ptr(), out.scale.data_ptr())
+    _check(lib().fvsr_quantize_fp8(rows, cols, x.data_ptr(), _dtype_code(x), 1 if square else 0,
+                                   *((None, None) + held if transpose else held + (None, None)), _here(x)))
     return out
 
 
 def quantize_fp8_both(x, square: bool = False, stream=None) -> tuple:
     """(quantize_fp8(x), quantize_fp8(x, transpose=True)) from one pass over x."""
     x = _matrix(x, "x")
+    away = _elsewhere(x, stream)
+    if away is not None:
+        with away:
+            return quantize_fp8_both(x, square)
     rows, cols = x.shape
-    if rows == 0:
-        raise FVSRError(FVSR_EINVAL, "the transpose of a tensor without rows has no form")
-    with _Launch(x.device, stream) as st:
-        out, out_t = Fp8Tensor.empty(rows, cols, x.device), Fp8Tensor.empty(cols, rows, x.device)
-        _check(lib().fvsr_quantize_fp8(rows, cols, _ptr(x), _dtype_code(x), int(bool(square)), _ptr(out.data),
-                                       _ptr(out.scale), _ptr(out_t.data), _ptr(out_t.scale), st))
+    if rows == 0 or cols == 0:
+        raise FVSRError(FVSR_EINVAL, f"a tensor of {(rows, cols)} has no 8-bit form both ways")
+    out, out_t = Fp8Tensor.empty_like(x, rows, cols), Fp8Tensor.empty_like(x, cols, rows)
+    _check(lib().fvsr_quantize_fp8(rows, cols, x.data_ptr(), _dtype_code(x), 1 if square else 0, out.data.data_ptr(),
+                                   out.scale.data_ptr(), out_t.data.data_ptr(), out_t.scale.data_ptr(), _here(x)))
     return out, out_t
 
 
 def dequantize_fp8(t: Fp8Tensor, dtype=None, out=None, stream=None):
     """The values of an 8-bit tensor as bf16 (the default) or fp32 (fvsr_dequantize_fp8)."""
-    torch = _torch()
-    with _Launch(t.device, stream) as st:
-        if out is None:
-            out = torch.empty((t.rows, t.cols), dtype=dtype or torch.bfloat16, device=t.device)
-        out = _matrix(out, "out", shape=t.shape, device=t.device)
-        if dtype is not None and out.dtype != dtype:
-            raise FVSRError(FVSR_EINVAL, f"out must be {dtype}")
-        _check(lib().fvsr_dequantize_fp8(t.rows, t.cols, _ptr(t.data), _ptr(t.scale), _ptr(out), _dtype_code(out), st))
+    away = _elsewhere(t.data, stream)
+    if away is not None:
+        with away:
+            return dequantize_fp8(t, dtype, out)
+    if out is None:
+        out = t.data.new_empty((t.rows, t.cols), dtype=dtype or _torch().bfloat16)
+    out = _matrix(out, "out", shape=t.shape, like=t.data)
+    if dtype is not None and out.dtype != dtype:
+        raise FVSRError(FVSR_EINVAL, f"out must be {dtype}")
+    _check(lib().fvsr_dequantize_fp8(t.rows, t.cols, t.data.data_ptr(), t.scale.data_ptr(), out.data_ptr(),
+                                     _dtype_code(out), _here(out)))
     return out
 
 
@@ -857,61 +897,56 @@ def linear_fp8(x, w: Fp8Tensor, bias=None, epilogue: int = FVSR_LINEAR, gate=Non
     a uint8 tensor of linear_fp8_workspace_size(...) bytes, else it is allocated."""
     torch = _torch()
     held = isinstance(x, Fp8Tensor)
-    if not held:
-        x = _matrix(x, "x", dtypes=(torch.bfloat16,))
+    xt = x.data if held else _matrix(x, "x", dtypes=(torch.bfloat16,))
     if not isinstance(w, Fp8Tensor):
         raise FVSRError(FVSR_EINVAL, "w must be an Fp8Tensor")
-    (m, k), n, dev = x.shape, w.rows, w.device
-    if w.cols != k or x.device != dev:
-        raise FVSRError(FVSR_EINVAL, f"w must be ({n}, {k}) on {x.device}")
-    _channel_vector(bias, "bias", n, torch.bfloat16, dev)
-    _channel_vector(gate, "gate", n, torch.bfloat16, dev)
+    away = _elsewhere(xt, stream)
+    if away is not None:
+        with away:
+            return linear_fp8(x, w, bias, epilogue, gate, resid, out, out_dtype, workspace)
+    (m, k), n = x.shape if held else xt.shape, w.rows
+    if w.cols != k or n < 1 or w.data.get_device() != xt.get_device():
+        raise FVSRError(FVSR_EINVAL, f"w must be (N, {k}) on {xt.device}, got {w.shape} on {w.device}")
+    bias = _channel_vector(bias, "bias", n, torch.bfloat16, xt)
+    gate = _channel_vector(gate, "gate", n, torch.bfloat16, xt)
     if out is not None:
-        out = _matrix(out, "out", shape=(m, n), device=dev)
-        out_dtype = out_dtype or out.dtype
-    out_dtype = out_dtype or torch.bfloat16
-    if out is not None and out.dtype != out_dtype:
-        raise FVSRError(FVSR_EINVAL, f"out must be {out_dtype}")
+        out = _matrix(out, "out", shape=(m, n), like=xt)
+    elif out_dtype is None or out_dtype == torch.bfloat16 or out_dtype == torch.float32:
+        out = xt.new_empty((m, n), dtype=out_dtype or torch.bfloat16)
+    if out is None or (out_dtype is not None and out.dtype != out_dtype):
+        raise FVSRError(FVSR_EINVAL, f"out must be bfloat16 or float32 as out_dtype says, got {out_dtype}")
     if resid is not None:
-        resid = _matrix(resid, "resid", dtypes=(out_dtype,), shape=(m, n), device=dev)
-    with _Launch(dev, stream) as st:
-        if out is None:
-            if out_dtype not in (torch.bfloat16, torch.float32):
-                raise FVSRError(FVSR_EINVAL, f"out must be bfloat16 or float32, got {out_dtype}")
-            out = torch.empty((m, n), dtype=out_dtype, device=dev)
-        need = linear_fp8_workspace_size(m, n, k, held) if workspace is None else 0
-        if need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-        xp, xs = (_ptr(x.data), _ptr(x.scale)) if held else (_ptr(x), None)
-        _check(lib().fvsr_linear_fp8(m, n, k, xp, xs, _ptr(w.data), _ptr(w.scale), _ptr(bias), int(epilogue),
-                                     _ptr(gate), _ptr(resid), _ptr(out), _dtype_code(out), _ptr(workspace),
-                                     0 if workspace is None else workspace.numel(), st))
+        resid = _matrix(resid, "resid", dtypes=(out.dtype,), shape=(m, n), like=xt).data_ptr()
+    need = linear_fp8_workspace_size(m, n, k, held) if workspace is None else 0
+    ws, ws_bytes, workspace = _scratch(workspace, need, xt)
+    _check(lib().fvsr_linear_fp8(m, n, k, xt.data_ptr(), x.scale.data_ptr() if held else None, w.data.data_ptr(),
+                                 w.scale.data_ptr(), bias, epilogue, gate, resid, out.data_ptr(), _dtype_code(out), ws,
+                                 ws_bytes, _here(xt)))
     return out
 
 
 def linear_fp8_workspace_size(m: int, n: int, k: int, x_is_fp8: bool) -> int:
-    size = ctypes.c_size_t(0)
-    _check(lib().fvsr_linear_fp8_workspace_size(m, n, k, int(x_is_fp8), ctypes.byref(size)))
-    return size.value
+    """Bytes of workspace of a linear_fp8 call on the current device."""
+    device = _torch().cuda.current_device() if _torch().cuda.is_available() else -1
+    return _bytes("fvsr_linear_fp8_workspace_size", device, m, n, k, 1 if x_is_fp8 else 0)
 
 
 def layernorm_train(x, weight=None, bias=None, shift=None, scale=None, eps: float = 1e-6, out=None, stream=None):
     """LayerNorm's forward pass for training (fvsr_layernorm_train): (out, mean, rstd) with n = (x - mean) * rstd and
     out = (n * weight + bias) * (1 + scale) + shift; x (M, C) bf16 or fp32, the vectors (C) like x, mean and rstd (M)
     fp32 for layernorm_backward."""
-    torch = _torch()
     x = _matrix(x, "x")
-    m, c = x.shape
-    for t, name in ((weight, "weight"), (bias, "bias"), (shift, "shift"), (scale, "scale")):
-        _channel_vector(t, name, c, x.dtype, x.device)
-    if out is not None:
-        out = _matrix(out, "out", dtypes=(x.dtype,), shape=(m, c), device=x.device)
-    with _Launch(x.device, stream) as st:
-        if out is None:
-            out = torch.empty_like(x)
-        mean, rstd = torch.empty((2, m), dtype=torch.float32, device=x.device).unbind(0)
-        _check(lib().fvsr_layernorm_train(m, c, _ptr(x), _dtype_code(x), _ptr(weight), _ptr(bias), _ptr(shift),
-                                          _ptr(scale), float(eps), _ptr(out), _ptr(mean), _ptr(rstd), st))
+    away = _elsewhere(x, stream)
+    if away is not None:
+        with away:
+            return layernorm_train(x, weight, bias, shift, scale, eps, out)
+    (m, c), dt, f32 = x.shape, x.dtype, _torch().float32
+    weight, bias = _channel_vector(weight, "weight", c, dt, x), _channel_vector(bias, "bias", c, dt, x)
+    shift, scale = _channel_vector(shift, "shift", c, dt, x), _channel_vector(scale, "scale", c, dt, x)
+    out = _torch().empty_like(x) if out is None else _matrix(out, "out", dtypes=(dt,), shape=x.shape, like=x)
+    mean, rstd = x.new_empty((m,), dtype=f32), x.new_empty((m,), dtype=f32)
+    _check(lib().fvsr_layernorm_train(m, c, x.data_ptr(), _dtype_code(x), weight, bias, shift, scale, eps,
+                                      out.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _here(x)))
     return out, mean, rstd
 
 
@@ -919,38 +954,32 @@ def layernorm_backward(dy, x, mean, rstd, weight=None, bias=None, scale=None, dx
     """LayerNorm's backward pass (fvsr_layernorm_backward): x the forward's input, in dy's dtype or as an Fp8Tensor (its
     8-bit form); weight, bias and scale as the forward had them. Returns {"dx", "dweight", "dbias", "dscale",
     "dshift"}: dx (M, C) like dy, the vectors' gradients (C) fp32, None where the forward had no such vector."""
-    torch = _torch()
     dy = _matrix(dy, "dy")
-    m, c = dy.shape
-    dev = dy.device
-    held = isinstance(x, Fp8Tensor)
-    if held:
-        if x.shape != (m, c) or x.device != dev:
-            raise FVSRError(FVSR_EINVAL, f"x must be ({m}, {c}) on {dev}")
+    away = _elsewhere(dy, stream)
+    if away is not None:
+        with away:
+            return layernorm_backward(dy, x, mean, rstd, weight, bias, scale, dx, workspace)
+    (m, c), dt, f32 = dy.shape, dy.dtype, _torch().float32
+    if isinstance(x, Fp8Tensor):
+        if x.shape != (m, c) or x.data.get_device() != dy.get_device():
+            raise FVSRError(FVSR_EINVAL, f"x must be ({m}, {c}) on {dy.device}, got {x.shape} on {x.device}")
+        xp, xs = x.data.data_ptr(), x.scale.data_ptr()
     else:
-        x = _matrix(x, "x", dtypes=(dy.dtype,), shape=(m, c), device=dev)
-    _channel_vector(mean, "mean", m, torch.float32, dev)
-    _channel_vector(rstd, "rstd", m, torch.float32, dev)
-    for t, name in ((weight, "weight"), (bias, "bias"), (scale, "scale")):
-        _channel_vector(t, name, c, dy.dtype, dev)
-    if dx is not None:
-        dx = _matrix(dx, "dx", dtypes=(dy.dtype,), shape=(m, c), device=dev)
-    with _Launch(dev, stream) as st:
-        if dx is None:
-            dx = torch.empty_like(dy)
-        kinds = (["dweight", "dbias"] if weight is not None else []) + (["dscale", "dshift"] if scale is not None else [])
-        grads = dict(zip(kinds, torch.empty((len(kinds), c), dtype=torch.float32, device=dev).unbind(0))) if kinds else {}
-        if workspace is None:
-            size = ctypes.c_size_t(0)
-            _check(lib().fvsr_layernorm_backward_workspace_size(m, c, ctypes.byref(size)))
-            workspace = torch.empty(size.value, dtype=torch.uint8, device=dev) if size.value else None
-        g = {k: grads.get(k) for k in ("dweight", "dbias", "dscale", "dshift")}
-        xp, xs = (_ptr(x.data), _ptr(x.scale)) if held else (_ptr(x), None)
-        _check(lib().fvsr_layernorm_backward(m, c, _ptr(dy), _dtype_code(dy), xp, xs, _ptr(mean), _ptr(rstd),
-                                             _ptr(weight), _ptr(bias), _ptr(scale), _ptr(dx), _ptr(g["dweight"]),
-                                             _ptr(g["dbias"]), _ptr(g["dscale"]), _ptr(g["dshift"]), _ptr(workspace),
-                                             0 if workspace is None else workspace.numel(), st))
-    return {"dx": dx, **g}
+        xp, xs = _matrix(x, "x", dtypes=(dt,), shape=dy.shape, like=dy).data_ptr(), None
+    mean, rstd = _channel_vector(mean, "mean", m, f32, dy), _channel_vector(rstd, "rstd", m, f32, dy)
+    if mean is None or rstd is None:
+        raise FVSRError(FVSR_EINVAL, "mean and rstd are required")
+    grads = {"dx": _torch().empty_like(dy) if dx is None else _matrix(dx, "dx", dtypes=(dt,), shape=dy.shape, like=dy)}
+    for name, given in (("dweight", weight), ("dbias", weight), ("dscale", scale), ("dshift", scale)):
+        grads[name] = None if given is None else dy.new_empty((c,), dtype=f32)
+    weight, bias = _channel_vector(weight, "weight", c, dt, dy), _channel_vector(bias, "bias", c, dt, dy)
+    scale = _channel_vector(scale, "scale", c, dt, dy)
+    need = _bytes("fvsr_layernorm_backward_workspace_size", dy.get_device(), m, c) if workspace is None else 0
+    ws, ws_bytes, workspace = _scratch(workspace, need, dy)
+    _check(lib().fvsr_layernorm_backward(m, c, dy.data_ptr(), _dtype_code(dy), xp, xs, mean, rstd, weight, bias, scale,
+                                         *(None if t is None else t.data_ptr() for t in grads.values()), ws, ws_bytes,
+                                         _here(dy)))
+    return grads
 
 
 def rope_tables(f: int, h: int, w: int, t0: int = 0, head_dim: int = 128, theta: float = 10000.0, device="cuda"):

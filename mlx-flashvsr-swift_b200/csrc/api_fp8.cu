@@ -95,6 +95,17 @@ fvsr_status fvsr_fp8_bytes(int64_t rows, int64_t cols, size_t* value_bytes, size
     return FVSR_OK;
 }
 
+fvsr_status fvsr_fp8_codes(int64_t rows, int64_t cols, const void* scale, void* out, fvsr_stream_t stream) {
+    fvsr_status s = check_held_shape(rows, cols);
+    if (s != FVSR_OK) return s;
+    if (rows == 0) return FVSR_OK;
+    if (!scale || !out) return refuse(FVSR_EINVAL, "scale and out are required");
+    if (!aligned(scale, 16)) return refuse(FVSR_EINVAL, "scale must be 16-byte aligned");
+    if ((s = check_device()) != FVSR_OK) return s;
+    return launched(launch_fp8_codes(rows, cols, static_cast<const uint8_t*>(scale), static_cast<uint8_t*>(out),
+                                     reinterpret_cast<cudaStream_t>(stream)), "codes launch");
+}
+
 fvsr_status fvsr_quantize_fp8(int64_t rows, int64_t cols, const void* x, int32_t dtype, int32_t square, void* q,
                               void* scale, void* qt, void* scale_t, fvsr_stream_t stream) {
     fvsr_status s = check_held_shape(rows, cols);

@@ -60,11 +60,20 @@ __device__ __forceinline__ float load_as_float(const __nv_bfloat16* p) { return 
 __device__ __forceinline__ void store_from_float(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_from_float(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
+// Multiprocessors of the current device.
+inline int sm_count() {
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+        return 148;
+    return n;
+}
+
 // ---- launchers ----
 // x (rows, cols) fp32 or bf16 → its 8-bit form (q, scale) and / or the 8-bit form of its transpose (qt, scale_t);
 // either pair may be NULL. square: one scale for each 128 × 128 square instead of each row's 128 values.
 cudaError_t launch_quantize_fp8(int64_t rows, int64_t cols, const void* x, int dtype, bool square, uint8_t* q,
                                 uint8_t* scale, uint8_t* qt, uint8_t* scale_t, cudaStream_t st);
+cudaError_t launch_fp8_codes(int64_t rows, int64_t cols, const uint8_t* scale, uint8_t* out, cudaStream_t st);
 cudaError_t launch_dequantize_fp8(int64_t rows, int64_t cols, const uint8_t* q, const uint8_t* scale, void* out,
                                   int dtype, cudaStream_t st);
 

@@ -320,13 +320,6 @@ __global__ void __launch_bounds__(256) gemm_fp8_join_kernel(const Fp8GemmArgs a,
     }
 }
 
-int sm_count() {
-    int dev = 0, n = 148;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-        n = 148;
-    return n;
-}
-
 template <typename T, int kMode>
 cudaError_t launch_tiles(const Fp8GemmArgs& args, const Work& wk, const CUtensorMap (&maps)[4], cudaStream_t st) {
     auto kernel = gemm_fp8_sm100_kernel<T, kMode>;

@@ -8,9 +8,11 @@
 // Both passes are bound by memory, x (and dy) read once and the result written once. A thread owns eight neighbouring
 // channels of every row it meets, so the vectors, and in the backward pass the sums A and B of those channels, stay in
 // its registers over all rows: tpr = ⌈c / 8⌉ threads, in whole warps, work on a row, kRows rows at once to share a
-// barrier, and the loads of the next kRows rows are in flight meanwhile. Narrow rows put several such groups in a CTA.
-// The variance is taken about the mean in a second pass over the registers. The vectors' gradients are summed per group
-// over its rows, then over the groups by a second kernel, both in a fixed order, so they do not depend on timing.
+// barrier; narrow rows put several such groups in a CTA. Rows are copied ahead into shared memory with cp.async, each
+// thread its own pieces (so that no barrier guards them), kStages sets of rows deep: what is in flight costs no
+// registers. Arithmetic is on pairs (f32x2), without which the backward pass would be bound by issue slots. The variance
+// is taken about the mean in a second pass over the pieces. The vectors' gradients are summed per group over its rows,
+// then over the groups by a second kernel, both in a fixed order, so they do not depend on timing.
 #include "../../include/fvsr_lcsa.h"
 #include "common.cuh"
 #include "fp8.cuh"
@@ -20,59 +22,94 @@ namespace fvsr {
 
 namespace {
 
-using sm100::bf2_to_f;
-using sm100::pack_bf16x2;
+using namespace sm100;
 
-// Eight values of a row as loaded: 16 bytes of bf16, 32 of fp32.
+__device__ __forceinline__ void copy_async16(void* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_async8(void* dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kPending>
+__device__ __forceinline__ void copy_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
+}
+
+// Eight values of a row as stored: 16 bytes of bf16, 32 of fp32. In shared memory a piece is split into 16-byte words,
+// [word][thread], so that a warp's accesses are contiguous.
 template <typename T>
-struct Raw8 {
-    uint4 u[sizeof(T) / 2];
+struct Piece {
+    static constexpr int kWords = (int)sizeof(T) / 2;
 };
 
-// Whole and 16-byte aligned (kVec), or element by element with zeros beyond n values.
+// The piece of n (0 to 8) values at p into words w[0], w[stride], …: whole pieces (kVec: 16-byte aligned) asynchronously,
+// else element by element with zeros beyond n.
 template <typename T, bool kVec>
-__device__ __forceinline__ void load8(const T* p, int n, Raw8<T>& r) {
-    if (kVec) {
+__device__ __forceinline__ void fetch8(const T* p, int n, uint4* w, int stride) {
+    if constexpr (kVec) {
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.u[i] = reinterpret_cast<const uint4*>(p)[i];
+        for (int i = 0; i < Piece<T>::kWords; ++i) {
+            if (n > 0) copy_async16(w + i * stride, reinterpret_cast<const uint4*>(p) + i);
+            else w[i * stride] = make_uint4(0, 0, 0, 0);
+        }
     } else {
         alignas(16) T v[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : T(0.0f);
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.u[i] = reinterpret_cast<const uint4*>(v)[i];
+        for (int i = 0; i < Piece<T>::kWords; ++i) w[i * stride] = reinterpret_cast<const uint4*>(v)[i];
     }
 }
-__device__ __forceinline__ void as_floats(const Raw8<__nv_bfloat16>& r, float (&f)[8]) {
-    bf2_to_f(r.u[0].x, f[0], f[1]), bf2_to_f(r.u[0].y, f[2], f[3]);
-    bf2_to_f(r.u[0].z, f[4], f[5]), bf2_to_f(r.u[0].w, f[6], f[7]);
+// A piece as four fp32 pairs.
+__device__ __forceinline__ uint64_t bf_pair(uint32_t u) {
+    float lo, hi;
+    bf2_to_f(u, lo, hi);
+    return f2(lo, hi);
 }
-__device__ __forceinline__ void as_floats(const Raw8<float>& r, float (&f)[8]) {
-    f[0] = __uint_as_float(r.u[0].x), f[1] = __uint_as_float(r.u[0].y);
-    f[2] = __uint_as_float(r.u[0].z), f[3] = __uint_as_float(r.u[0].w);
-    f[4] = __uint_as_float(r.u[1].x), f[5] = __uint_as_float(r.u[1].y);
-    f[6] = __uint_as_float(r.u[1].z), f[7] = __uint_as_float(r.u[1].w);
+__device__ __forceinline__ void pairs(const uint4* w, int, uint64_t (&f)[4], const __nv_bfloat16*) {
+    const uint4 u = *w;
+    f[0] = bf_pair(u.x), f[1] = bf_pair(u.y), f[2] = bf_pair(u.z), f[3] = bf_pair(u.w);
+}
+__device__ __forceinline__ void pairs(const uint4* w, int stride, uint64_t (&f)[4], const float*) {
+    const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(w), b = *reinterpret_cast<const ulonglong2*>(w + stride);
+    f[0] = a.x, f[1] = a.y, f[2] = b.x, f[3] = b.y;
+}
+__device__ __forceinline__ uint32_t pack_pair(uint64_t v) {
+    float lo, hi;
+    uf2(v, lo, hi);
+    return pack_bf16x2(lo, hi);
+}
+__device__ __forceinline__ float pair_sum(uint64_t v) {
+    float lo, hi;
+    uf2(v, lo, hi);
+    return lo + hi;
 }
 template <bool kVec>
-__device__ __forceinline__ void store8(__nv_bfloat16* p, int n, const float (&f)[8]) {
+__device__ __forceinline__ void store8(__nv_bfloat16* p, int n, const uint64_t (&f)[4]) {
     if (kVec) {
-        *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]),
-                                                  pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+        *reinterpret_cast<uint4*>(p) = make_uint4(pack_pair(f[0]), pack_pair(f[1]), pack_pair(f[2]), pack_pair(f[3]));
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < n) p[i] = __float2bfloat16_rn(f[i]);
+        for (int i = 0; i < 8; ++i) {
+            float v[2];
+            uf2(f[i >> 1], v[0], v[1]);
+            if (i < n) p[i] = __float2bfloat16_rn(v[i & 1]);
+        }
     }
 }
 template <bool kVec>
-__device__ __forceinline__ void store8(float* p, int n, const float (&f)[8]) {
+__device__ __forceinline__ void store8(float* p, int n, const uint64_t (&f)[4]) {
     if (kVec) {
-        reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
-        reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+        reinterpret_cast<ulonglong2*>(p)[0] = make_ulonglong2(f[0], f[1]);
+        reinterpret_cast<ulonglong2*>(p)[1] = make_ulonglong2(f[2], f[3]);
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < n) p[i] = f[i];
+        for (int i = 0; i < 8; ++i) {
+            float v[2];
+            uf2(f[i >> 1], v[0], v[1]);
+            if (i < n) p[i] = v[i & 1];
+        }
     }
 }
 
@@ -81,179 +118,271 @@ __device__ __forceinline__ float vec_or(const void* v, int c, float otherwise) {
     return v ? load_as_float(static_cast<const T*>(v) + c) : otherwise;
 }
 
-// The sums of v[0..N) over the tpr threads of a row group, in each of them: shuffles, then the warps' sums through
-// `part` ([32 warps][N]) and a barrier of the CTA (every thread calls this the same number of times; two calls in a row
-// use different buffers). In the order of the warps.
+// The sums of v[0..N) over the tpr threads of a row group, in each of them (N = 1, 2 or 4). Within a warp a butterfly
+// whose first steps also halve the values a lane holds; then the warps' sums through `part` ([32 warps][N]) and a barrier
+// of the CTA (every thread calls this the same number of times; two calls in a row use different buffers), which each
+// warp adds up by another butterfly. The order is fixed by the lanes.
 template <int N>
 __device__ __forceinline__ void group_sum(float (&v)[N], float* part, int group_warp0, int warps) {
+    const int lane = threadIdx.x & 31;
+    int bit = 16;
 #pragma unroll
-    for (int i = 0; i < N; ++i)
+    for (int half = N / 2; half >= 1; half /= 2, bit /= 2) {
+        const bool up = lane & bit;
 #pragma unroll
-        for (int o = 16; o >= 1; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
-    if (warps == 1) return;
-    if ((threadIdx.x & 31) == 0) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) part[(threadIdx.x >> 5) * N + i] = v[i];
+        for (int i = 0; i < half; ++i) {
+            const float keep = up ? v[i + half] : v[i], give = up ? v[i] : v[i + half];
+            v[i] = keep + __shfl_xor_sync(0xffffffffu, give, bit);
+        }
     }
+    constexpr int kHold = 32 / N;  // lanes that now hold the same value, lane / kHold
+    float s = v[0];
+#pragma unroll
+    for (int o = kHold / 2; o >= 1; o /= 2) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (warps == 1) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = __shfl_sync(0xffffffffu, s, i * kHold);
+        return;
+    }
+    if (lane % kHold == 0) part[(threadIdx.x >> 5) * N + lane / kHold] = s;
     __syncthreads();
+    part += group_warp0 * N;
+    s = lane < warps * N ? part[lane] : 0.0f;
+    for (int i = lane + 32; i < warps * N; i += 32) s += part[i];
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = 0.0f;
-    for (int w = 0; w < warps; ++w)
+    for (int o = 16; o >= N; o /= 2) s += __shfl_xor_sync(0xffffffffu, s, o);
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] += part[(group_warp0 + w) * N + i];
+    for (int i = 0; i < N; ++i) v[i] = __shfl_sync(0xffffffffu, s, i);
 }
 
+// 1 / √v: the hardware's approximation (2^-22) and one Newton step, except where that step has nothing to refine.
+__device__ __forceinline__ float rsqrt_refined(float v) {
+    const float r = rsqrtf(v);
+    return v > 0.0f && r > 0.0f ? r * fmaf(-0.5f * v * r, r, 1.5f) : r;
+}
+
+constexpr int kStages = 3;
+// Rows at once: forward four of bf16, two of fp32, backward two; one for more than kWideC channels, where a CTA's 1024
+// threads have 64 registers each. Threads that the kernels' registers let an SM hold: 768 of the forward pass (80
+// registers), 576 of the backward pass (112; 512 in CTAs of 256).
+constexpr int kWideC = 4096, kBackwardRows = 2, kForwardThreads = 768, kBackwardThreads = 576;
+
 template <typename T, bool kVec, int kRows, int kMaxThreads>
-__global__ void __launch_bounds__(kMaxThreads) norm_train_kernel(const NormTrainArgs a, int tpr) {
+__global__ void __launch_bounds__(kMaxThreads, kForwardThreads / kMaxThreads > 1 ? kForwardThreads / kMaxThreads : 1)
+    norm_train_kernel(const NormTrainArgs a, int tpr) {
+    extern __shared__ uint4 ring[];  // [kStages][kRows][words][kMaxThreads]
     __shared__ alignas(16) float part[2][32 * kRows];
-    const int groups = (int)blockDim.x / tpr, g = (int)threadIdx.x / tpr, col = ((int)threadIdx.x % tpr) * 8;
-    const int n = max(0, min(8, a.c - col)), warps = tpr >> 5, warp0 = g * warps;
-    const int64_t step = (int64_t)gridDim.x * groups * kRows;
+    constexpr int W = Piece<T>::kWords, kRowWords = W * kMaxThreads;
+    const int groups = (int)blockDim.x / tpr, g = (int)threadIdx.x / tpr;
+    const int col = ((int)threadIdx.x % tpr) * 8, n = max(0, min(8, a.c - col)), warps = tpr >> 5, warp0 = g * warps;
+    const int step = (int)gridDim.x * groups * kRows, row_first = ((int)blockIdx.x * groups + g) * kRows, m = (int)a.m;
+    const int64_t c = a.c;
     const float inv_c = 1.0f / (float)a.c;
+    int left = m - row_first;  // rows from the group's next ones to the end
     const T* x = static_cast<const T*>(a.x);
-    T* out = static_cast<T*>(a.out);
-    griddep_wait_then_release();
-    float gain[8], base[8];
+    int64_t fetch_at = row_first * c + col;  // of the rows to fetch next
+    auto fetch = [&](uint4* to, int rows) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int c = col + (i < n ? i : 0);
-        const float s1 = n > 0 ? 1.0f + vec_or<T>(a.scale, c, 0.0f) : 0.0f;
-        gain[i] = n > 0 ? s1 * vec_or<T>(a.weight, c, 1.0f) : 0.0f;
-        base[i] = n > 0 ? fmaf(vec_or<T>(a.bias, c, 0.0f), s1, vec_or<T>(a.shift, c, 0.0f)) : 0.0f;
-    }
-    Raw8<T> next[kRows];
-    auto fetch = [&](int64_t row0) {
-#pragma unroll
-        for (int i = 0; i < kRows; ++i) {
-            next[i] = Raw8<T>{};
-            if (row0 + i < a.m && n > 0) load8<T, kVec>(x + (row0 + i) * a.c + col, n, next[i]);
-        }
+        for (int i = 0; i < kRows; ++i)
+            fetch8<T, kVec>(x + fetch_at + i * c, i < rows ? n : 0, to + i * kRowWords, kMaxThreads);
+        copy_async_commit();
+        fetch_at += step * c;
     };
-    int64_t row0 = ((int64_t)blockIdx.x * groups + g) * kRows;
-    fetch(row0);
-    for (int64_t cta0 = (int64_t)blockIdx.x * groups * kRows; cta0 < a.m; cta0 += step, row0 += step) {
-        Raw8<T> now[kRows];
-        float sum[kRows], sq[kRows], f[8];
+    griddep_wait_then_release();
+    uint4* const mine = ring + threadIdx.x;
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) fetch(mine + s * kRows * kRowWords, left - s * step);
+    uint64_t gain[4], base[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float gv[2], bv[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const bool here = 2 * i + j < n;
+            const int at = here ? col + 2 * i + j : 0;
+            const float s1 = 1.0f + vec_or<T>(a.scale, at, 0.0f);
+            gv[j] = here ? s1 * vec_or<T>(a.weight, at, 1.0f) : 0.0f;
+            bv[j] = here ? fmaf(vec_or<T>(a.bias, at, 0.0f), s1, vec_or<T>(a.shift, at, 0.0f)) : 0.0f;
+        }
+        gain[i] = f2(gv[0], gv[1]), base[i] = f2(bv[0], bv[1]);
+    }
+    int stage = 0;
+    for (int cta_left = m - (int)blockIdx.x * groups * kRows; cta_left > 0; cta_left -= step, left -= step) {
+        fetch(mine + (stage == 0 ? kStages - 1 : stage - 1) * kRows * kRowWords, left - (kStages - 1) * step);
+        copy_async_wait<kStages - 1>();
+        const uint4* now = mine + stage * kRows * kRowWords;
+        float sum[kRows], sq[kRows];
+        uint64_t f[kRows][4];
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
-            now[i] = next[i];
-            as_floats(now[i], f);
-            sum[i] = ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
+            pairs(now + i * kRowWords, kMaxThreads, f[i], x);
+            sum[i] = pair_sum(fadd2(fadd2(f[i][0], f[i][1]), fadd2(f[i][2], f[i][3])));
         }
-        fetch(row0 + step);
         group_sum<kRows>(sum, part[0], warp0, warps);
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
             sum[i] *= inv_c;
-            as_floats(now[i], f);
-            sq[i] = 0.0f;
+            const uint64_t minus = f2(-sum[i], -sum[i]);
+            uint64_t q = 0;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float d = f[j] - sum[i];
-                if (kVec ? n > 0 : j < n) sq[i] = fmaf(d, d, sq[i]);
+            for (int j = 0; j < 4; ++j) {
+                f[i][j] = fadd2(f[i][j], minus);
+                uint64_t d = f[i][j];
+                if (!kVec && 2 * j + 1 >= n) {  // a piece that ends inside
+                    float lo, hi;
+                    uf2(d, lo, hi);
+                    d = f2(2 * j < n ? lo : 0.0f, 0.0f);
+                }
+                q = ffma2(d, d, q);
             }
+            sq[i] = n > 0 ? pair_sum(q) : 0.0f;
         }
         group_sum<kRows>(sq, part[1], warp0, warps);
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
-            if (row0 + i >= a.m) break;
-            const float rstd = 1.0f / sqrtf(fmaf(sq[i], inv_c, a.eps));
-            if (col == 0) a.mean[row0 + i] = sum[i], a.rstd[row0 + i] = rstd;
+            if (i >= left) break;
+            const float rstd = rsqrt_refined(fmaf(sq[i], inv_c, a.eps));
+            if (col == 0) a.mean[m - left + i] = sum[i], a.rstd[m - left + i] = rstd;
             if (n == 0) continue;
-            as_floats(now[i], f);
+            const uint64_t r2 = f2(rstd, rstd);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) f[j] = fmaf((f[j] - sum[i]) * rstd, gain[j], base[j]);
-            store8<kVec>(out + (row0 + i) * a.c + col, n, f);
+            for (int j = 0; j < 4; ++j) f[i][j] = ffma2(fmul2(f[i][j], r2), gain[j], base[j]);
+            store8<kVec>(static_cast<T*>(a.out) + (int64_t)(m - left + i) * c + col, n, f[i]);
         }
+        stage = stage == kStages - 1 ? 0 : stage + 1;
     }
+    copy_async_wait<0>();
 }
 
-// kHeld: x is the 8-bit form.
+// kHeld: x is the 8-bit form; a piece of it is 8 bytes.
 template <typename T, bool kHeld, bool kVec, int kRows, int kMaxThreads>
-__global__ void __launch_bounds__(kMaxThreads) norm_backward_kernel(const NormTrainArgs a, int tpr) {
+__global__ void __launch_bounds__(kMaxThreads, kBackwardThreads / kMaxThreads > 1 ? kBackwardThreads / kMaxThreads : 1)
+    norm_backward_kernel(const NormTrainArgs a, int tpr) {
+    extern __shared__ uint4 ring[];  // [kStages][kRows][words of dy][kMaxThreads], then the same of x (8 bytes if held)
     __shared__ alignas(16) float part[2][32 * 2 * kRows];
-    const int groups = (int)blockDim.x / tpr, g = (int)threadIdx.x / tpr, col = ((int)threadIdx.x % tpr) * 8;
-    const int n = max(0, min(8, a.c - col)), warps = tpr >> 5, warp0 = g * warps;
-    const int64_t step = (int64_t)gridDim.x * groups * kRows, ld = fp8_ld(a.c), tiles = fp8_scale_tiles(a.c);
-    const float inv_c = 1.0f / (float)a.c;
-    const T *x = static_cast<const T*>(a.x), *dy = static_cast<const T*>(a.dy);
+    constexpr int W = Piece<T>::kWords, kRowWords = W * kMaxThreads;
+    const int groups = (int)blockDim.x / tpr, g = (int)threadIdx.x / tpr;
+    const int col = ((int)threadIdx.x % tpr) * 8, n = max(0, min(8, a.c - col)), warps = tpr >> 5, warp0 = g * warps;
+    const int step = (int)gridDim.x * groups * kRows, row_first = ((int)blockIdx.x * groups + g) * kRows, m = (int)a.m;
+    const int64_t c = a.c, ld = fp8_ld(a.c);
+    const float inv_c = -1.0f / (float)a.c;
+    int left = m - row_first;  // rows from the group's next ones to the end
+    const T *dy = static_cast<const T*>(a.dy), *x = static_cast<const T*>(a.x);
     const uint8_t* x8 = static_cast<const uint8_t*>(a.x);
-    T* dx = static_cast<T*>(a.out);
-    griddep_wait_then_release();
-    float gain[8], sum_a[8], sum_b[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int c = col + (i < n ? i : 0);
-        gain[i] = n > 0 ? (1.0f + vec_or<T>(a.scale, c, 0.0f)) * vec_or<T>(a.weight, c, 1.0f) : 0.0f;
-        sum_a[i] = sum_b[i] = 0.0f;
-    }
-    Raw8<T> next_dy[kRows], next_x[kHeld ? 1 : kRows];
-    uint2 next_x8[kHeld ? kRows : 1];
-    uint32_t next_code[kHeld ? kRows : 1];
-    float next_mean[kRows], next_rstd[kRows];
-    auto fetch = [&](int64_t row0) {
+    int64_t fetch_at = row_first * c + col, fetch_at8 = row_first * ld + col;  // of the rows to fetch next
+    uint4* const mine = ring + threadIdx.x;
+    uint4* const mine_x = mine + kStages * kRows * kRowWords;
+    uint2* const mine_x8 = reinterpret_cast<uint2*>(ring + kStages * kRows * kRowWords) + threadIdx.x;
+    auto fetch = [&](int stage, int rows) {
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
-            const int64_t r = row0 + i;
-            const bool here = r < a.m && n > 0;
-            next_dy[i] = Raw8<T>{};
-            if (here) load8<T, kVec>(dy + r * a.c + col, n, next_dy[i]);
+            const int here = i < rows ? n : 0;
+            fetch8<T, kVec>(dy + fetch_at + i * c, here, mine + (stage * kRows + i) * kRowWords, kMaxThreads);
             if constexpr (kHeld) {
-                next_x8[i] = here ? *reinterpret_cast<const uint2*>(x8 + r * ld + col) : make_uint2(0, 0);
-                next_code[i] = here ? a.x_scale[fp8_code_pos(r, col >> 7, tiles)] : 0u;
+                uint2* to = mine_x8 + (stage * kRows + i) * kMaxThreads;
+                if (here > 0) copy_async8(to, x8 + fetch_at8 + i * ld);
+                else *to = make_uint2(0, 0);
             } else {
-                next_x[i] = Raw8<T>{};
-                if (here) load8<T, kVec>(x + r * a.c + col, n, next_x[i]);
+                fetch8<T, kVec>(x + fetch_at + i * c, here, mine_x + (stage * kRows + i) * kRowWords, kMaxThreads);
             }
-            next_mean[i] = here ? a.mean[r] : 0.0f;
-            next_rstd[i] = here ? a.rstd[r] : 0.0f;
+        }
+        copy_async_commit();
+        fetch_at += step * c;
+        if (kHeld) fetch_at8 += step * ld;
+    };
+    // the rows' statistics (and codes) one step ahead, in registers
+    float next_mean[kRows], next_rstd[kRows];
+    uint32_t next_code[kRows];
+    auto fetch_row = [&](int rows) {
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            next_mean[i] = next_rstd[i] = 0.0f;
+            next_code[i] = 0;
+            if (i < rows) {
+                const int r = m - rows + i;
+                next_mean[i] = a.mean[r], next_rstd[i] = a.rstd[r];
+                if (kHeld && n > 0) next_code[i] = a.x_scale[fp8_code_pos(r, col >> 7, fp8_scale_tiles(a.c))];
+            }
         }
     };
-    int64_t row0 = ((int64_t)blockIdx.x * groups + g) * kRows;
-    fetch(row0);
-    int flip = 0;
-    for (int64_t cta0 = (int64_t)blockIdx.x * groups * kRows; cta0 < a.m; cta0 += step, row0 += step, flip ^= 1) {
-        float norm[kRows][8], grad[kRows][8], rstd[kRows], s[2 * kRows];
+    griddep_wait_then_release();
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) fetch(s, left - s * step);
+    fetch_row(left);
+    uint64_t gain[4], sum_a[4], sum_b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float gv[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const bool here = 2 * i + j < n;
+            const int at = here ? col + 2 * i + j : 0;
+            gv[j] = here ? (1.0f + vec_or<T>(a.scale, at, 0.0f)) * vec_or<T>(a.weight, at, 1.0f) : 0.0f;
+        }
+        gain[i] = f2(gv[0], gv[1]);
+        sum_a[i] = sum_b[i] = 0;
+    }
+    int stage = 0, flip = 0;
+    for (int cta_left = m - (int)blockIdx.x * groups * kRows; cta_left > 0; cta_left -= step, left -= step, flip ^= 1) {
+        fetch(stage == 0 ? kStages - 1 : stage - 1, left - (kStages - 1) * step);
+        copy_async_wait<kStages - 1>();
+        uint64_t norm[kRows][4], grad[kRows][4];
+        float rstd[kRows], s[2 * kRows];
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
             rstd[i] = next_rstd[i];
-            as_floats(next_dy[i], grad[i]);
+            pairs(mine + (stage * kRows + i) * kRowWords, kMaxThreads, grad[i], dy);
             if constexpr (kHeld) {
+                const uint2 u = mine_x8[(stage * kRows + i) * kMaxThreads];
+                const uint32_t two[4] = {u.x, u.x >> 16, u.y, u.y >> 16};
                 const float down = fp8_down(next_code[i]);
-                fp8_unpack2(next_x8[i].x, norm[i][0], norm[i][1]);
-                fp8_unpack2(next_x8[i].x >> 16, norm[i][2], norm[i][3]);
-                fp8_unpack2(next_x8[i].y, norm[i][4], norm[i][5]);
-                fp8_unpack2(next_x8[i].y >> 16, norm[i][6], norm[i][7]);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) norm[i][j] *= down;
+                for (int j = 0; j < 4; ++j) {
+                    float lo, hi;
+                    fp8_unpack2(two[j], lo, hi);
+                    norm[i][j] = fmul2(f2(lo, hi), f2(down, down));
+                }
             } else {
-                as_floats(next_x[i], norm[i]);
+                pairs(mine_x + (stage * kRows + i) * kRowWords, kMaxThreads, norm[i], dy);
             }
-            s[2 * i] = s[2 * i + 1] = 0.0f;
+            const uint64_t minus = f2(-next_mean[i], -next_mean[i]), r2 = f2(rstd[i], rstd[i]);
+            uint64_t s1 = 0, s2 = 0;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                norm[i][j] = (norm[i][j] - next_mean[i]) * rstd[i];
-                sum_a[j] = fmaf(grad[i][j], norm[i][j], sum_a[j]);
-                sum_b[j] += grad[i][j];
-                grad[i][j] *= gain[j];
-                s[2 * i] += grad[i][j];
-                s[2 * i + 1] = fmaf(grad[i][j], norm[i][j], s[2 * i + 1]);
+            for (int j = 0; j < 4; ++j) {
+                norm[i][j] = fmul2(fadd2(norm[i][j], minus), r2);
+                sum_a[j] = ffma2(grad[i][j], norm[i][j], sum_a[j]);
+                sum_b[j] = fadd2(sum_b[j], grad[i][j]);
+                grad[i][j] = fmul2(grad[i][j], gain[j]);
+                s1 = fadd2(s1, grad[i][j]);
+                s2 = ffma2(grad[i][j], norm[i][j], s2);
             }
+            s[2 * i] = pair_sum(s1), s[2 * i + 1] = n > 0 ? pair_sum(s2) : 0.0f;
         }
-        fetch(row0 + step);
+        fetch_row(left - step);
         group_sum<2 * kRows>(s, part[flip], warp0, warps);
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
-            if (row0 + i >= a.m || n == 0) break;
+            if (i >= left || n == 0) break;
             const float c1 = s[2 * i] * inv_c, c2 = s[2 * i + 1] * inv_c;
-            float f[8];
+            const uint64_t c1p = f2(c1, c1), c2p = f2(c2, c2), r2 = f2(rstd[i], rstd[i]);
+            uint64_t f[4];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) f[j] = rstd[i] * (grad[i][j] - c1 - norm[i][j] * c2);
-            store8<kVec>(dx + (row0 + i) * a.c + col, n, f);
+            for (int j = 0; j < 4; ++j) f[j] = fmul2(ffma2(norm[i][j], c2p, fadd2(grad[i][j], c1p)), r2);
+            store8<kVec>(static_cast<T*>(a.out) + (int64_t)(m - left + i) * c + col, n, f);
         }
+        stage = stage == kStages - 1 ? 0 : stage + 1;
     }
-    float* mine = a.partial + ((int64_t)blockIdx.x * groups + g) * 2 * a.c + col;
-    for (int i = 0; i < n; ++i) mine[i] = sum_a[i], mine[a.c + i] = sum_b[i];
+    copy_async_wait<0>();
+    float* to = a.partial + ((int64_t)blockIdx.x * groups + g) * 2 * a.c + col;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float av[2], bv[2];
+        uf2(sum_a[i], av[0], av[1]);
+        uf2(sum_b[i], bv[0], bv[1]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+            if (2 * i + j < n) to[2 * i + j] = av[j], to[a.c + 2 * i + j] = bv[j];
+    }
 }
 
 // The groups' sums of 32 channels: 32 rows of threads take every 32nd group each, then their sums in order.
@@ -283,41 +412,46 @@ __global__ void __launch_bounds__(1024) norm_vectors_kernel(const NormTrainArgs 
     if (a.dshift) a.dshift[c] = vb;
 }
 
-int sm_count() {
-    int dev = 0, n = 148;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-        n = 148;
-    return n;
-}
-
-// Threads of a row and of a CTA for c channels, and how many CTAs fit an SM at `regs` registers a thread.
+// Threads of a row and of a CTA for c channels, and how many CTAs share an SM.
 struct Shape {
     int tpr, threads, groups;
     explicit Shape(int c) : tpr(((c + 7) / 8 + 31) / 32 * 32), groups(tpr >= 256 ? 1 : 256 / tpr) { threads = tpr * groups; }
-    int per_sm(int regs) const { const int n = 65536 / regs / threads; return n < 1 ? 1 : n; }
+    int most_threads() const { return threads <= 192 ? 192 : threads <= 256 ? 256 : threads <= 512 ? 512 : 1024; }
+    int ctas(int64_t m, int rows, int sm_threads) const {
+        const int64_t need = (m + groups * rows - 1) / (groups * rows);
+        const int64_t most = (int64_t)sm_count() * (sm_threads > threads ? sm_threads / threads : 1);
+        return (int)(need < most ? need : most);
+    }
 };
-int ctas_for(int64_t m, const Shape& s, int rows, int regs) {
-    const int64_t need = (m + s.groups * rows - 1) / (s.groups * rows), most = (int64_t)sm_count() * s.per_sm(regs);
-    return (int)(need < most ? need : most);
+template <typename Kernel>
+cudaError_t launch_ring(Kernel kernel, int ctas, const Shape& s, size_t ring_bytes, const NormTrainArgs& a, cudaStream_t st) {
+    if (ring_bytes > 40 * 1024) {
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ring_bytes);
+        if (e != cudaSuccess) return e;
+    }
+    return launch_pdl(kernel, dim3(ctas), dim3(s.threads), ring_bytes, st, a, s.tpr);
 }
-// Rows at once: forward four of bf16, two of fp32, backward two; one where 1024 threads leave 64 registers each.
-constexpr int kWideC = 4096, kBackwardRows = 2;
 
 template <typename T, bool kVec>
 cudaError_t train(const NormTrainArgs& a, cudaStream_t st) {
     constexpr int kRows = sizeof(T) == 2 ? 4 : 2;
     const Shape s(a.c);
-    const dim3 grid(ctas_for(a.m, s, a.c > kWideC ? 1 : kRows, 64)), block(s.threads);
-    if (a.c > kWideC) return launch_pdl(norm_train_kernel<T, kVec, 1, 1024>, grid, block, 0, st, a, s.tpr);
-    return launch_pdl(norm_train_kernel<T, kVec, kRows, 512>, grid, block, 0, st, a, s.tpr);
+    const int rows = a.c > kWideC ? 1 : kRows, ctas = s.ctas(a.m, rows, kForwardThreads);
+    const size_t ring = (size_t)kStages * rows * s.most_threads() * 8 * sizeof(T);
+    if (s.threads <= 192) return launch_ring(norm_train_kernel<T, kVec, kRows, 192>, ctas, s, ring, a, st);
+    if (s.threads <= 256) return launch_ring(norm_train_kernel<T, kVec, kRows, 256>, ctas, s, ring, a, st);
+    if (a.c <= kWideC) return launch_ring(norm_train_kernel<T, kVec, kRows, 512>, ctas, s, ring, a, st);
+    return launch_ring(norm_train_kernel<T, kVec, 1, 1024>, ctas, s, ring, a, st);
 }
 
 template <typename T, bool kHeld, bool kVec>
 cudaError_t backward_rows(const NormTrainArgs& a, const Shape& s, int ctas, cudaStream_t st) {
     constexpr int kRows = kBackwardRows;
-    const dim3 grid(ctas), block(s.threads);
-    if (a.c > kWideC) return launch_pdl(norm_backward_kernel<T, kHeld, kVec, 1, 1024>, grid, block, 0, st, a, s.tpr);
-    return launch_pdl(norm_backward_kernel<T, kHeld, kVec, kRows, 512>, grid, block, 0, st, a, s.tpr);
+    const size_t ring = (size_t)kStages * (a.c > kWideC ? 1 : kRows) * s.most_threads() * 8 * (sizeof(T) + (kHeld ? 1 : sizeof(T)));
+    if (s.threads <= 192) return launch_ring(norm_backward_kernel<T, kHeld, kVec, kRows, 192>, ctas, s, ring, a, st);
+    if (s.threads <= 256) return launch_ring(norm_backward_kernel<T, kHeld, kVec, kRows, 256>, ctas, s, ring, a, st);
+    if (a.c <= kWideC) return launch_ring(norm_backward_kernel<T, kHeld, kVec, kRows, 512>, ctas, s, ring, a, st);
+    return launch_ring(norm_backward_kernel<T, kHeld, kVec, 1, 1024>, ctas, s, ring, a, st);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -342,7 +476,7 @@ cudaError_t backward(const NormTrainArgs& a, cudaStream_t st) {
 
 int64_t norm_backward_groups(int64_t m, int c) {
     const Shape s(c);
-    return (int64_t)ctas_for(m, s, c > kWideC ? 1 : kBackwardRows, 128) * s.groups;
+    return (int64_t)s.ctas(m, c > kWideC ? 1 : kBackwardRows, kBackwardThreads) * s.groups;
 }
 
 cudaError_t launch_layernorm_train(const NormTrainArgs& a, cudaStream_t st) {

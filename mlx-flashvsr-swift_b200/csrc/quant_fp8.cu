@@ -3,9 +3,11 @@
 // of the 8-bit linear layers (blocks along the channels for the forward and input-gradient products, blocks along the
 // tokens for the weight gradient, 128 × 128 squares for weights, whose transpose has the same scales).
 //
-// Both directions move bytes and do little else. quantize_kernel: one CTA of 8 warps per 128 × 128 tile, which each warp
-// reads 16 rows of with 128-bit loads, all in flight at once, and keeps in registers; a row's largest magnitude is a
-// shuffle over the lanes that hold it. The row form is written from the registers. For the transposed form the tile goes
+// Both directions move bytes, and the instructions spent on each decide how near they come to memory's rate.
+// quantize_kernel: one CTA of 8 warps per 128 × 128 tile, which each warp reads 16 rows of with 128-bit loads, all in
+// flight at once, and keeps in registers. The rows' largest magnitudes are found together: a butterfly in which each step
+// halves the rows a lane still holds (8 shuffles for 16 rows instead of 32), after which a row's code is computed once
+// and handed back with one shuffle. The row form is written from the registers. For the transposed form the tile goes
 // through shared memory once, as stored: a warp then owns 32 rows and a lane two neighbouring columns of them, so that
 // reads are free of bank conflicts and a lane writes 32 consecutive bytes of each of its two lines. Either way x is read
 // once for both forms.
@@ -18,10 +20,10 @@ namespace fvsr {
 
 namespace {
 
-using sm100::bf2_to_f;
-using sm100::pack_bf16x2;
+using namespace sm100;
 
 constexpr int kT = 128, kThreads = 256;
+constexpr uint32_t kAbs = 0x7FFFFFFFu, kAbs2 = 0x7FFF7FFFu;
 
 // Elements of T in a 16-byte load, as the pieces of a tile row a lane holds.
 template <typename T>
@@ -32,41 +34,51 @@ struct Piece {
     static constexpr int kLoads = 16 / kRowsPerLoad;        // loads for a warp's 16 rows
 };
 
-__device__ __forceinline__ void unpack(const uint4& u, float (&f)[8], const __nv_bfloat16*) {
-    bf2_to_f(u.x, f[0], f[1]), bf2_to_f(u.y, f[2], f[3]), bf2_to_f(u.z, f[4], f[5]), bf2_to_f(u.w, f[6], f[7]);
-}
-__device__ __forceinline__ void unpack(const uint4& u, float (&f)[4], const float*) {
-    f[0] = __uint_as_float(u.x), f[1] = __uint_as_float(u.y), f[2] = __uint_as_float(u.z), f[3] = __uint_as_float(u.w);
-}
 // The largest magnitude of a piece, as fp32 bits (an integer maximum: a NaN's bits are above infinity's).
 __device__ __forceinline__ uint32_t piece_max(const uint4& u, const __nv_bfloat16*) {
-    const uint32_t m = 0x7FFF7FFFu;
-    const uint32_t a = __vmaxu2(__vmaxu2(u.x & m, u.y & m), __vmaxu2(u.z & m, u.w & m));
+    const uint32_t a = __vmaxu2(__vmaxu2(u.x & kAbs2, u.y & kAbs2), __vmaxu2(u.z & kAbs2, u.w & kAbs2));
     return max(a & 0xFFFF0000u, a << 16);
 }
 __device__ __forceinline__ uint32_t piece_max(const uint4& u, const float*) {
-    const uint32_t m = 0x7FFFFFFFu;
-    return max(max(u.x & m, u.y & m), max(u.z & m, u.w & m));
+    return max(max(u.x & kAbs, u.y & kAbs), max(u.z & kAbs, u.w & kAbs));
 }
-
-__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
-    return fp8_pack2(a, b) | (fp8_pack2(c, d) << 16);
+// Four values, as two pairs already scaled, in e4m3.
+__device__ __forceinline__ uint32_t pack4(uint64_t a, uint64_t b) {
+    float x, y, z, w;
+    uf2(a, x, y);
+    uf2(b, z, w);
+    return fp8_pack2(x, y) | (fp8_pack2(z, w) << 16);
+}
+__device__ __forceinline__ uint64_t bf_pair(uint32_t u) {
+    float lo, hi;
+    bf2_to_f(u, lo, hi);
+    return f2(lo, hi);
+}
+__device__ __forceinline__ void put_piece(uint8_t* p, const uint4& u, uint64_t up, const __nv_bfloat16*) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack4(fmul2(bf_pair(u.x), up), fmul2(bf_pair(u.y), up)),
+                                              pack4(fmul2(bf_pair(u.z), up), fmul2(bf_pair(u.w), up)));
+}
+__device__ __forceinline__ void put_piece(uint8_t* p, const uint4& u, uint64_t up, const float*) {
+    const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&u);
+    *reinterpret_cast<uint32_t*>(p) = pack4(fmul2(v.x, up), fmul2(v.y, up));
 }
 
 // kVec: rows are 16-byte aligned and their lengths whole pieces; else element by element.
 template <typename T, bool kVec>
-__device__ __forceinline__ uint4 load_piece(const T* row, int64_t c, int64_t cols) {
-    if (kVec) return c < cols ? __ldcs(reinterpret_cast<const uint4*>(row + c)) : make_uint4(0, 0, 0, 0);
-    alignas(16) T v[Piece<T>::kElems];
+__device__ __forceinline__ uint4 load_piece(const T* p, int left) {
+    if constexpr (kVec) {
+        return left > 0 ? __ldcs(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
+    } else {
+        alignas(16) T v[Piece<T>::kElems];
 #pragma unroll
-    for (int i = 0; i < Piece<T>::kElems; ++i) v[i] = c + i < cols ? row[c + i] : T(0.0f);
-    return *reinterpret_cast<const uint4*>(v);
+        for (int i = 0; i < Piece<T>::kElems; ++i) v[i] = i < left ? p[i] : T(0.0f);
+        return *reinterpret_cast<const uint4*>(v);
+    }
 }
 
-// The codes of a line (form row) beyond its last block, up to the end of the last tile of codes, are zero.
+// The code of a line (form row); those beyond its last block, up to the end of the last tile of codes, are zero.
 __device__ __forceinline__ void put_code(uint8_t* scale, int64_t line, int64_t block, int64_t blocks, uint32_t code) {
-    const int64_t tiles = (blocks + 3) >> 2;
-    uint8_t* p = scale + fp8_code_pos(line, block, tiles);
+    uint8_t* p = scale + fp8_code_pos(line, block, (blocks + 3) >> 2);
     *p = (uint8_t)code;
     if (block == blocks - 1)
         for (int i = 1; i < 4 - (int)(block & 3); ++i) p[i] = 0;
@@ -80,78 +92,76 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(int64_t rows, int64_
     using P = Piece<T>;
     extern __shared__ uint4 tile4[];  // kTrans: the tile, [128][128] of T
     __shared__ uint32_t warp_max[kThreads / 32], col_max[4][kT];
-    griddep_wait_then_release();
-    const int64_t ct = (cols + kT - 1) / kT, rt = (rows + kT - 1) / kT;
-    const int64_t rb = blockIdx.x / ct, cb = blockIdx.x % ct, r0 = rb * kT, c0 = cb * kT;
+    const uint32_t ct = (uint32_t)((cols + kT - 1) / kT);
+    const uint32_t rb = blockIdx.x / ct, cb = blockIdx.x % ct;
+    const int64_t r0 = (int64_t)rb * kT, c0 = (int64_t)cb * kT;
+    const int nr = (int)min((int64_t)kT, rows - r0), nc = (int)min((int64_t)kT, cols - c0);  // of the tile
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int sub = lane / P::kLanes, piece = lane % P::kLanes;
+    const int sub = lane / P::kLanes, c = lane % P::kLanes * P::kElems, row = warp * 16 + sub;  // row of load 0
+    griddep_wait_then_release();
     uint4 v[P::kLoads];
+    const T* src = x + (r0 + row) * cols + c0 + c;
 #pragma unroll
-    for (int i = 0; i < P::kLoads; ++i) {
-        const int64_t r = r0 + warp * 16 + i * P::kRowsPerLoad + sub;
-        v[i] = r < rows ? load_piece<T, kVec>(x + r * cols, c0 + piece * P::kElems, cols) : make_uint4(0, 0, 0, 0);
-    }
+    for (int i = 0; i < P::kLoads; ++i)
+        v[i] = load_piece<T, kVec>(src + (int64_t)(i * P::kRowsPerLoad) * cols, row + i * P::kRowsPerLoad < nr ? nc - c : 0);
     uint32_t top[P::kLoads];
 #pragma unroll
     for (int i = 0; i < P::kLoads; ++i) {
         top[i] = piece_max(v[i], x);
-#pragma unroll
-        for (int o = P::kLanes / 2; o >= 1; o >>= 1) top[i] = max(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
-        if (kTrans) tile4[(warp * 16 + i * P::kRowsPerLoad + sub) * P::kLanes + piece] = v[i];
+        if (kTrans) tile4[(row + i * P::kRowsPerLoad) * P::kLanes + lane % P::kLanes] = v[i];
     }
-    if (square) {
-        uint32_t m = top[0];
+    // After the butterfly the lanes 2i and 2i + 1 of a row's lanes hold the maximum of load i's row.
 #pragma unroll
-        for (int i = 1; i < P::kLoads; ++i) m = max(m, top[i]);
-        m = __reduce_max_sync(0xffffffffu, m);
-        if (lane == 0) warp_max[warp] = m;
+    for (int half = P::kLoads / 2, bit = P::kLanes / 2; half >= 1; half /= 2, bit /= 2) {
+        const bool up = lane & bit;
+#pragma unroll
+        for (int i = 0; i < half; ++i) {
+            const uint32_t keep = up ? top[i + half] : top[i], give = up ? top[i] : top[i + half];
+            top[i] = max(keep, __shfl_xor_sync(0xffffffffu, give, bit));
+        }
+    }
+    uint32_t most = max(top[0], __shfl_xor_sync(0xffffffffu, top[0], 1));
+    if (square) {
+        most = __reduce_max_sync(0xffffffffu, most);
+        if (lane == 0) warp_max[warp] = most;
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < kThreads / 32; ++i) m = max(m, warp_max[i]);
-#pragma unroll
-        for (int i = 0; i < P::kLoads; ++i) top[i] = m;
+        for (int i = 0; i < kThreads / 32; ++i) most = max(most, warp_max[i]);
     }
     if (q) {
-        const int64_t ld = ct * kT;
+        const uint32_t code = fp8_code(most);
+        const float up = fp8_up(code);
+        const int64_t ld = (int64_t)ct * kT;
+        uint8_t* dst = q + (r0 + row) * ld + c0 + c;
 #pragma unroll
         for (int i = 0; i < P::kLoads; ++i) {
-            const int64_t r = r0 + warp * 16 + i * P::kRowsPerLoad + sub;
-            const uint32_t code = fp8_code(top[i]);
-            const float up = fp8_up(code);
-            float f[P::kElems];
-            unpack(v[i], f, x);
-            if (r < rows) {
-                uint8_t* p = q + r * ld + c0 + piece * P::kElems;
-                if constexpr (P::kElems == 8)
-                    *reinterpret_cast<uint2*>(p) = make_uint2(pack4(f[0] * up, f[1] * up, f[2] * up, f[3] * up),
-                                                              pack4(f[4] * up, f[5] * up, f[6] * up, f[7] * up));
-                else
-                    *reinterpret_cast<uint32_t*>(p) = pack4(f[0] * up, f[1] * up, f[2] * up, f[3] * up);
-            }
-            if (piece == 0) put_code(scale, r, cb, ct, r < rows ? code : 0u);
+            const float u = __shfl_sync(0xffffffffu, up, (lane & ~(P::kLanes - 1)) | (2 * i));
+            if (row + i * P::kRowsPerLoad < nr) put_piece(dst + (int64_t)(i * P::kRowsPerLoad) * ld, v[i], f2(u, u), x);
         }
+        const int mine = row + (lane % P::kLanes >> 1) * P::kRowsPerLoad;
+        if (!(lane & 1)) put_code(scale, r0 + mine, cb, ct, mine < nr ? code : 0u);
     }
     if constexpr (kTrans) {
         // lane: columns 2·cp, 2·cp + 1 of the 32 rows [32·quarter, +32)
         __syncthreads();
         const int quarter = warp & 3, cp = (warp >> 2) * 32 + lane;
-        const int64_t ld = rt * kT;
-        float a[32], b[32];
-        uint32_t ma = 0, mb = 0;
+        const int64_t rt = (rows + kT - 1) / kT, ld = rt * kT;
         const T* tile = reinterpret_cast<const T*>(tile4) + (quarter * 32) * kT + 2 * cp;
+        uint32_t ma = 0, mb = 0;
+        uint64_t w[32];  // a row's two columns: a bf16 pair in the low half, or two fp32
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
             if constexpr (sizeof(T) == 2) {
-                bf2_to_f(*reinterpret_cast<const uint32_t*>(tile + i * kT), a[i], b[i]);
+                w[i] = *reinterpret_cast<const uint32_t*>(tile + i * kT);
+                ma = __vmaxu2(ma, (uint32_t)w[i] & kAbs2);
             } else {
-                const float2 t = *reinterpret_cast<const float2*>(tile + i * kT);
-                a[i] = t.x, b[i] = t.y;
+                w[i] = *reinterpret_cast<const uint64_t*>(tile + i * kT);
+                ma = max(ma, (uint32_t)w[i] & kAbs), mb = max(mb, (uint32_t)(w[i] >> 32) & kAbs);
             }
-            ma = max(ma, __float_as_uint(a[i]) & 0x7FFFFFFFu);
-            mb = max(mb, __float_as_uint(b[i]) & 0x7FFFFFFFu);
         }
+        if constexpr (sizeof(T) == 2) mb = ma & 0xFFFF0000u, ma <<= 16;
         if (square) {
-            ma = mb = top[0];
+            ma = mb = most;
         } else {
             *reinterpret_cast<uint2*>(&col_max[quarter][2 * cp]) = make_uint2(ma, mb);
             __syncthreads();
@@ -161,22 +171,27 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(int64_t rows, int64_
                 ma = max(ma, m.x), mb = max(mb, m.y);
             }
         }
-        const int64_t line = c0 + 2 * cp;
         const uint32_t code_a = fp8_code(ma), code_b = fp8_code(mb);
-        auto emit = [&](const float (&f)[32], float up, int64_t l) {
-            uint32_t w[8];
+        const uint64_t up = f2(fp8_up(code_a), fp8_up(code_b));
+        uint32_t a[8], b[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                w[i] = pack4(f[4 * i] * up, f[4 * i + 1] * up, f[4 * i + 2] * up, f[4 * i + 3] * up);
-            uint4* p = reinterpret_cast<uint4*>(qt + l * ld + r0 + quarter * 32);
-            p[0] = make_uint4(w[0], w[1], w[2], w[3]);
-            p[1] = make_uint4(w[4], w[5], w[6], w[7]);
-        };
-        if (line < cols) emit(a, fp8_up(code_a), line);
-        if (line + 1 < cols) emit(b, fp8_up(code_b), line + 1);
+        for (int i = 0; i < 8; ++i) {
+            float fa[4], fb[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint64_t p = w[4 * i + j];
+                uf2(fmul2(sizeof(T) == 2 ? bf_pair((uint32_t)p) : p, up), fa[j], fb[j]);
+            }
+            a[i] = fp8_pack2(fa[0], fa[1]) | (fp8_pack2(fa[2], fa[3]) << 16);
+            b[i] = fp8_pack2(fb[0], fb[1]) | (fp8_pack2(fb[2], fb[3]) << 16);
+        }
+        uint4* p = reinterpret_cast<uint4*>(qt + (c0 + 2 * cp) * ld + r0 + quarter * 32);
+        if (2 * cp < nc) p[0] = make_uint4(a[0], a[1], a[2], a[3]), p[1] = make_uint4(a[4], a[5], a[6], a[7]);
+        p = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(p) + ld);
+        if (2 * cp + 1 < nc) p[0] = make_uint4(b[0], b[1], b[2], b[3]), p[1] = make_uint4(b[4], b[5], b[6], b[7]);
         if (quarter == 0) {
-            put_code(scale_t, line, rb, rt, line < cols ? code_a : 0u);
-            put_code(scale_t, line + 1, rb, rt, line + 1 < cols ? code_b : 0u);
+            put_code(scale_t, c0 + 2 * cp, rb, rt, 2 * cp < nc ? code_a : 0u);
+            put_code(scale_t, c0 + 2 * cp + 1, rb, rt, 2 * cp + 1 < nc ? code_b : 0u);
         }
     }
 }
@@ -190,8 +205,8 @@ __global__ void __launch_bounds__(kThreads) dequantize_kernel(int64_t rows, int6
     griddep_wait_then_release();
     const int64_t ld = fp8_ld(cols), tiles = fp8_scale_tiles(cols);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t items = (rows + kRows - 1) / kRows * tiles;
-    for (int64_t it = (int64_t)blockIdx.x * (kThreads / 32) + warp; it < items; it += (int64_t)gridDim.x * (kThreads / 32)) {
+    const int64_t it = (int64_t)blockIdx.x * (kThreads / 32) + warp;
+    {
         const int64_t tile = it % tiles, r0 = it / tiles * kRows, c = tile * 512 + lane * 16;
         uint4 v[kRows];
         uint32_t word[kRows];
@@ -233,11 +248,16 @@ __global__ void __launch_bounds__(kThreads) dequantize_kernel(int64_t rows, int6
     }
 }
 
-int sm_count() {
-    int dev = 0, n = 148;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-        n = 148;
-    return n;
+// A thread takes one row's four codes of a tile.
+__global__ void __launch_bounds__(kThreads) codes_kernel(int64_t rows, int64_t blocks, const uint8_t* __restrict__ scale,
+                                                         uint8_t* __restrict__ out) {
+    griddep_wait_then_release();
+    const int64_t tiles = (blocks + 3) >> 2, items = rows * tiles;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < items; i += (int64_t)gridDim.x * kThreads) {
+        const int64_t r = i / tiles, b = i % tiles * 4;
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(scale + fp8_code_pos(r, b, tiles));
+        for (int j = 0; j < 4 && b + j < blocks; ++j) out[r * blocks + b + j] = (uint8_t)(w >> (8 * j));
+    }
 }
 
 template <typename T, bool kVec, bool kTrans>
@@ -267,8 +287,8 @@ cudaError_t quantize_t(int64_t rows, int64_t cols, const T* x, bool square, uint
 template <typename T>
 cudaError_t dequantize_t(int64_t rows, int64_t cols, const uint8_t* q, const uint8_t* scale, T* out, cudaStream_t st) {
     const bool vec = cols % Piece<T>::kElems == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
-    const int64_t items = (rows + 3) / 4 * fp8_scale_tiles(cols), blocks = (items + 7) / 8, most = (int64_t)sm_count() * 8;
-    const dim3 grid((unsigned)(blocks < most ? blocks : most));
+    const int64_t items = (rows + 3) / 4 * fp8_scale_tiles(cols);
+    const dim3 grid((unsigned)((items + 7) / 8));
     return vec ? launch_pdl(dequantize_kernel<T, true>, grid, dim3(kThreads), 0, st, rows, cols, q, scale, out)
                : launch_pdl(dequantize_kernel<T, false>, grid, dim3(kThreads), 0, st, rows, cols, q, scale, out);
 }
@@ -280,6 +300,12 @@ cudaError_t launch_quantize_fp8(int64_t rows, int64_t cols, const void* x, int d
     return dtype == FVSR_BF16
                ? quantize_t(rows, cols, static_cast<const __nv_bfloat16*>(x), square, q, scale, qt, scale_t, st)
                : quantize_t(rows, cols, static_cast<const float*>(x), square, q, scale, qt, scale_t, st);
+}
+
+cudaError_t launch_fp8_codes(int64_t rows, int64_t cols, const uint8_t* scale, uint8_t* out, cudaStream_t st) {
+    const int64_t need = (rows * fp8_scale_tiles(cols) + kThreads - 1) / kThreads, most = (int64_t)sm_count() * 8;
+    return launch_pdl(codes_kernel, dim3((unsigned)(need < most ? need : most)), dim3(kThreads), 0, st, rows,
+                      (cols + 127) / 128, scale, out);
 }
 
 cudaError_t launch_dequantize_fp8(int64_t rows, int64_t cols, const uint8_t* q, const uint8_t* scale, void* out,
