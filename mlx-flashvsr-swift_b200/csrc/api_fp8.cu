@@ -217,7 +217,7 @@ fvsr_status fvsr_layernorm_backward_workspace_size(int64_t m, int32_t c, size_t*
     fvsr_status s = check_norm(m, c, FVSR_F32);
     if (s != FVSR_OK) return s;
     if (!bytes) return refuse(FVSR_EINVAL, "bytes is NULL");
-    *bytes = (size_t)norm_backward_groups(m, c) * 2 * (size_t)c * sizeof(float);
+    *bytes = (size_t)norm_backward_ctas(m, c) * 2 * (size_t)c * sizeof(float);
     return FVSR_OK;
 }
 

@@ -111,12 +111,12 @@ struct NormTrainArgs {
     float *mean, *rstd;
     const void* dy;
     float *dweight, *dbias, *dshift, *dscale;
-    float* partial;                  // norm_backward_groups × 2 × c
+    float* partial;                  // norm_backward_ctas × 2 × c
 };
 cudaError_t launch_layernorm_train(const NormTrainArgs& a, cudaStream_t st);
 cudaError_t launch_layernorm_backward(const NormTrainArgs& a, cudaStream_t st);
-// Row groups of the backward pass, each leaving 2 · c partial sums.
-int64_t norm_backward_groups(int64_t m, int c);
+// CTAs of the backward pass, each leaving 2 · c partial sums.
+int norm_backward_ctas(int64_t m, int c);
 constexpr int kNormTrainMaxC = 8192;
 
 }  // namespace fvsr

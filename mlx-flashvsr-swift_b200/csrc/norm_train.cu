@@ -11,8 +11,8 @@
 // barrier; narrow rows put several such groups in a CTA. Rows are copied ahead into shared memory with cp.async, each
 // thread its own pieces (so that no barrier guards them), kStages sets of rows deep: what is in flight costs no
 // registers. Arithmetic is on pairs (f32x2), without which the backward pass would be bound by issue slots. The variance
-// is taken about the mean in a second pass over the pieces. The vectors' gradients are summed per group over its rows,
-// then over the groups by a second kernel, both in a fixed order, so they do not depend on timing.
+// is taken about the mean in a second pass over the pieces. The vectors' gradients are summed per CTA over its rows,
+// then over the CTAs by a second kernel, both in a fixed order, so they do not depend on timing.
 #include "../../include/fvsr_lcsa.h"
 #include "common.cuh"
 #include "fp8.cuh"
@@ -331,25 +331,28 @@ __global__ void __launch_bounds__(kMaxThreads, kBackwardThreads / kMaxThreads > 
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
             rstd[i] = next_rstd[i];
+            const uint64_t minus = f2(-next_mean[i], -next_mean[i]);
             pairs(mine + (stage * kRows + i) * kRowWords, kMaxThreads, grad[i], dy);
             if constexpr (kHeld) {
                 const uint2 u = mine_x8[(stage * kRows + i) * kMaxThreads];
                 const uint32_t two[4] = {u.x, u.x >> 16, u.y, u.y >> 16};
                 const float down = fp8_down(next_code[i]);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int j = 0; j < 4; ++j) {  // the scaling is exact: one rounding, in the subtraction
                     float lo, hi;
                     fp8_unpack2(two[j], lo, hi);
-                    norm[i][j] = fmul2(f2(lo, hi), f2(down, down));
+                    norm[i][j] = ffma2(f2(lo, hi), f2(down, down), minus);
                 }
             } else {
                 pairs(mine_x + (stage * kRows + i) * kRowWords, kMaxThreads, norm[i], dy);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) norm[i][j] = fadd2(norm[i][j], minus);
             }
-            const uint64_t minus = f2(-next_mean[i], -next_mean[i]), r2 = f2(rstd[i], rstd[i]);
+            const uint64_t r2 = f2(rstd[i], rstd[i]);
             uint64_t s1 = 0, s2 = 0;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                norm[i][j] = fmul2(fadd2(norm[i][j], minus), r2);
+                norm[i][j] = fmul2(norm[i][j], r2);
                 sum_a[j] = ffma2(grad[i][j], norm[i][j], sum_a[j]);
                 sum_b[j] = fadd2(sum_b[j], grad[i][j]);
                 grad[i][j] = fmul2(grad[i][j], gain[j]);
@@ -373,7 +376,28 @@ __global__ void __launch_bounds__(kMaxThreads, kBackwardThreads / kMaxThreads > 
         stage = stage == kStages - 1 ? 0 : stage + 1;
     }
     copy_async_wait<0>();
-    float* to = a.partial + ((int64_t)blockIdx.x * groups + g) * 2 * a.c + col;
+    // the CTA's sums: the groups' in order, through the ring
+    if (groups > 1) {
+        __syncthreads();
+        ulonglong2* const held = reinterpret_cast<ulonglong2*>(ring);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            held[i * kMaxThreads + threadIdx.x] = make_ulonglong2(sum_a[2 * i], sum_a[2 * i + 1]);
+            held[(2 + i) * kMaxThreads + threadIdx.x] = make_ulonglong2(sum_b[2 * i], sum_b[2 * i + 1]);
+        }
+        __syncthreads();
+        for (int o = 1; g == 0 && o < groups; ++o) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const ulonglong2 va = held[i * kMaxThreads + threadIdx.x + o * tpr];
+                const ulonglong2 vb = held[(2 + i) * kMaxThreads + threadIdx.x + o * tpr];
+                sum_a[2 * i] = fadd2(sum_a[2 * i], va.x), sum_a[2 * i + 1] = fadd2(sum_a[2 * i + 1], va.y);
+                sum_b[2 * i] = fadd2(sum_b[2 * i], vb.x), sum_b[2 * i + 1] = fadd2(sum_b[2 * i + 1], vb.y);
+            }
+        }
+        if (g != 0) return;
+    }
+    float* to = a.partial + (int64_t)blockIdx.x * 2 * a.c + col;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         float av[2], bv[2];
@@ -385,26 +409,37 @@ __global__ void __launch_bounds__(kMaxThreads, kBackwardThreads / kMaxThreads > 
     }
 }
 
-// The groups' sums of 32 channels: 32 rows of threads take every 32nd group each, then their sums in order.
+// The CTAs' sums of eight channels (a 32-byte sector): 64 rows of eight threads take every 64th CTA's each, eight at a
+// time in flight (the few hundred CTAs of a full device are one round trip to L2), then their sums in a fixed order.
 template <typename T>
-__global__ void __launch_bounds__(1024) norm_vectors_kernel(const NormTrainArgs a, int groups) {
-    __shared__ float sa[32][33], sb[32][33];
+__global__ void __launch_bounds__(512) norm_vectors_kernel(const NormTrainArgs a, int ctas) {
+    __shared__ float sa[16][8], sb[16][8];
     griddep_wait_then_release();
-    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, c = blockIdx.x * 32 + tx;
+    const int tx = threadIdx.x & 7, ty = threadIdx.x >> 3, c = blockIdx.x * 8 + tx;
     float va = 0.0f, vb = 0.0f;
-    if (c < a.c) {
-#pragma unroll 4
-        for (int i = ty; i < groups; i += 32) {
-            va += a.partial[(int64_t)i * 2 * a.c + c];
-            vb += a.partial[((int64_t)i * 2 + 1) * a.c + c];
+    const int64_t step = (int64_t)128 * a.c;
+    const float* p = a.partial + (int64_t)ty * 2 * a.c + c;
+    for (int i = c < a.c ? ty : ctas; i < ctas; i += 512) {
+        float pa[8], pb[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j, p += step) {
+            const bool here = i + 64 * j < ctas;
+            pa[j] = here ? p[0] : 0.0f, pb[j] = here ? p[a.c] : 0.0f;
         }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) va += pa[j], vb += pb[j];
     }
-    sa[ty][tx] = va, sb[ty][tx] = vb;
+#pragma unroll
+    for (int o = 8; o <= 16; o *= 2) {
+        va += __shfl_xor_sync(0xffffffffu, va, o);
+        vb += __shfl_xor_sync(0xffffffffu, vb, o);
+    }
+    if ((threadIdx.x & 31) < 8) sa[threadIdx.x >> 5][tx] = va, sb[threadIdx.x >> 5][tx] = vb;
     __syncthreads();
     if (ty != 0 || c >= a.c) return;
     va = vb = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) va += sa[i][tx], vb += sb[i][tx];
+    for (int i = 0; i < 16; ++i) va += sa[i][tx], vb += sb[i][tx];
     const float s1 = 1.0f + vec_or<T>(a.scale, c, 0.0f);
     if (a.dweight) a.dweight[c] = s1 * va;
     if (a.dbias) a.dbias[c] = s1 * vb;
@@ -459,7 +494,7 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 template <typename T>
 cudaError_t backward(const NormTrainArgs& a, cudaStream_t st) {
     const Shape s(a.c);
-    const int groups = (int)norm_backward_groups(a.m, a.c), ctas = groups / s.groups;
+    const int ctas = norm_backward_ctas(a.m, a.c);
     cudaError_t e = cudaSuccess;
     if (ctas > 0) {
         const bool vec = a.c % 8 == 0 && aligned16(a.dy) && aligned16(a.out) && aligned16(a.x);
@@ -469,14 +504,13 @@ cudaError_t backward(const NormTrainArgs& a, cudaStream_t st) {
             e = vec ? backward_rows<T, false, true>(a, s, ctas, st) : backward_rows<T, false, false>(a, s, ctas, st);
     }
     if (e != cudaSuccess || !(a.dweight || a.dbias || a.dscale || a.dshift)) return e;
-    return launch_pdl(norm_vectors_kernel<T>, dim3((a.c + 31) / 32), dim3(1024), 0, st, a, groups);
+    return launch_pdl(norm_vectors_kernel<T>, dim3((a.c + 7) / 8), dim3(512), 0, st, a, ctas);
 }
 
 }  // namespace
 
-int64_t norm_backward_groups(int64_t m, int c) {
-    const Shape s(c);
-    return (int64_t)s.ctas(m, c > kWideC ? 1 : kBackwardRows, kBackwardThreads) * s.groups;
+int norm_backward_ctas(int64_t m, int c) {
+    return Shape(c).ctas(m, c > kWideC ? 1 : kBackwardRows, kBackwardThreads);
 }
 
 cudaError_t launch_layernorm_train(const NormTrainArgs& a, cudaStream_t st) {

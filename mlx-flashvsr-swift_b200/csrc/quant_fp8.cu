@@ -11,6 +11,8 @@
 // through shared memory once, as stored: a warp then owns 32 rows and a lane two neighbouring columns of them, so that
 // reads are free of bank conflicts and a lane writes 32 consecutive bytes of each of its two lines. Either way x is read
 // once for both forms.
+#include <type_traits>
+
 #include "../../include/fvsr_lcsa.h"
 #include "common.cuh"
 #include "fp8.cuh"
@@ -32,6 +34,7 @@ struct Piece {
     static constexpr int kLanes = kT / kElems;              // lanes of a row
     static constexpr int kRowsPerLoad = 32 / kLanes;        // rows a warp covers with one load
     static constexpr int kLoads = 16 / kRowsPerLoad;        // loads for a warp's 16 rows
+    using Held = std::conditional_t<sizeof(T) == 2, uint2, uint32_t>;  // the piece in 8 bits
 };
 
 // The largest magnitude of a piece, as fp32 bits (an integer maximum: a NaN's bits are above infinity's).
@@ -185,10 +188,22 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(int64_t rows, int64_
             a[i] = fp8_pack2(fa[0], fa[1]) | (fp8_pack2(fa[2], fa[3]) << 16);
             b[i] = fp8_pack2(fb[0], fb[1]) | (fp8_pack2(fb[2], fb[3]) << 16);
         }
-        uint4* p = reinterpret_cast<uint4*>(qt + (c0 + 2 * cp) * ld + r0 + quarter * 32);
-        if (2 * cp < nc) p[0] = make_uint4(a[0], a[1], a[2], a[3]), p[1] = make_uint4(a[4], a[5], a[6], a[7]);
-        p = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(p) + ld);
-        if (2 * cp + 1 < nc) p[0] = make_uint4(b[0], b[1], b[2], b[3]), p[1] = make_uint4(b[4], b[5], b[6], b[7]);
+        // Neighbouring lanes swap halves, so that one store of a warp fills whole 32-byte sectors: of the lines of the
+        // even lane (then of the odd one) the even lane writes the first 16 bytes and the odd lane the rest.
+        const bool odd = lane & 1;
+        uint8_t* p = qt + (c0 + 2 * (cp & ~1)) * ld + r0 + quarter * 32 + (odd ? 16 : 0);
+        auto put = [&](const uint32_t (&v)[8], int line) {
+            uint32_t got[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) got[i] = __shfl_xor_sync(0xffffffffu, odd ? v[i] : v[4 + i], 1);
+            const uint4 mine = odd ? make_uint4(v[4], v[5], v[6], v[7]) : make_uint4(v[0], v[1], v[2], v[3]);
+            const uint4 theirs = make_uint4(got[0], got[1], got[2], got[3]);
+            const int first = 2 * (cp & ~1) + line;  // in the tile: the even lane's line, and two further the odd lane's
+            if (first < nc) *reinterpret_cast<uint4*>(p + line * ld) = odd ? theirs : mine;
+            if (first + 2 < nc) *reinterpret_cast<uint4*>(p + (line + 2) * ld) = odd ? mine : theirs;
+        };
+        put(a, 0);
+        put(b, 1);
         if (quarter == 0) {
             put_code(scale_t, c0 + 2 * cp, rb, rt, 2 * cp < nc ? code_a : 0u);
             put_code(scale_t, c0 + 2 * cp + 1, rb, rt, 2 * cp + 1 < nc ? code_b : 0u);
@@ -196,53 +211,59 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(int64_t rows, int64_
     }
 }
 
-// A warp takes 512 columns of a row: a lane 16 values, and the four codes of the row's tile as one word. kRows rows at
-// once keep enough loads in flight.
+// A warp takes 512 columns of four rows: a lane 16 bytes' worth of output at a time, next to its neighbours', and the four
+// codes of a row's tile as one word.
 template <typename T, bool kVec>
 __global__ void __launch_bounds__(kThreads) dequantize_kernel(int64_t rows, int64_t cols, const uint8_t* __restrict__ q,
                                                               const uint8_t* __restrict__ scale, T* __restrict__ out) {
-    constexpr int kRows = 4;
-    griddep_wait_then_release();
-    const int64_t ld = fp8_ld(cols), tiles = fp8_scale_tiles(cols);
+    constexpr int kRows = 4, kElems = Piece<T>::kElems, kSteps = 512 / (32 * kElems);
+    using Word = typename Piece<T>::Held;
+    const int64_t ld = fp8_ld(cols);
+    const uint32_t tiles = (uint32_t)fp8_scale_tiles(cols);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t it = (int64_t)blockIdx.x * (kThreads / 32) + warp;
-    {
-        const int64_t tile = it % tiles, r0 = it / tiles * kRows, c = tile * 512 + lane * 16;
-        uint4 v[kRows];
-        uint32_t word[kRows];
+    const uint64_t it = (uint64_t)blockIdx.x * (kThreads / 32) + warp;
+    const int64_t tile = it % tiles, r0 = it / tiles * kRows, c = tile * 512 + lane * kElems;
+    const int here = (int)min((int64_t)kRows, rows - r0), left = (int)min(cols - tile * 512, (int64_t)512) - lane * kElems;
+    griddep_wait_then_release();
+    Word v[kRows][kSteps];
+    uint32_t word[kRows];
 #pragma unroll
-        for (int i = 0; i < kRows; ++i) {
-            const bool here = r0 + i < rows && c < cols;
-            v[i] = here ? __ldcs(reinterpret_cast<const uint4*>(q + (r0 + i) * ld + c)) : make_uint4(0, 0, 0, 0);
-            word[i] = here ? *reinterpret_cast<const uint32_t*>(scale + fp8_code_pos(r0 + i, tile * 4, tiles)) : 0u;
+    for (int i = 0; i < kRows; ++i) {
+        const uint8_t* p = q + (r0 + i) * ld + c;
+        word[i] = i < here ? *reinterpret_cast<const uint32_t*>(scale + fp8_code_pos(r0 + i, tile * 4, tiles)) : 0u;
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j) {
+            v[i][j] = Word{};
+            if (i < here && j * 32 * kElems < left) v[i][j] = __ldcs(reinterpret_cast<const Word*>(p + j * 32 * kElems));
         }
+    }
 #pragma unroll
-        for (int i = 0; i < kRows; ++i) {
-            if (r0 + i >= rows || c >= cols) continue;
-            const float down = fp8_down((word[i] >> (8 * (lane >> 3))) & 255u);
-            const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-            float f[16];
+    for (int i = 0; i < kRows; ++i) {
+        if (i >= here) break;
+        T* p = out + (r0 + i) * cols + c;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                fp8_unpack2(w[j >> 1] >> (16 * (j & 1)), f[2 * j], f[2 * j + 1]);
-                f[2 * j] *= down, f[2 * j + 1] *= down;
+        for (int j = 0; j < kSteps; ++j) {
+            const int at = j * 32 * kElems;
+            if (at >= left) break;
+            const int block = (lane * kElems + at) >> 7;
+            const float down = fp8_down((word[i] >> (8 * block)) & 255u);
+            const uint32_t w[2] = {reinterpret_cast<const uint32_t*>(&v[i][j])[0],
+                                   kElems == 8 ? reinterpret_cast<const uint32_t*>(&v[i][j])[kElems == 8] : 0u};
+            float f[kElems];
+#pragma unroll
+            for (int e = 0; e < kElems; e += 2) {
+                fp8_unpack2(w[e >> 2] >> (16 * ((e >> 1) & 1)), f[e], f[e + 1]);
+                f[e] *= down, f[e + 1] *= down;
             }
-            T* p = out + (r0 + i) * cols + c;
-            if (kVec) {
-#pragma unroll
-                for (int j = 0; j < 16; j += Piece<T>::kElems) {
-                    if (c + j >= cols) break;
-                    if constexpr (sizeof(T) == 2)
-                        *reinterpret_cast<uint4*>(p + j) =
-                            make_uint4(pack_bf16x2(f[j], f[j + 1]), pack_bf16x2(f[j + 2], f[j + 3]),
-                                       pack_bf16x2(f[j + 4], f[j + 5]), pack_bf16x2(f[j + 6], f[j + 7]));
-                    else
-                        *reinterpret_cast<float4*>(p + j) = make_float4(f[j], f[j + 1], f[j + 2], f[j + 3]);
-                }
+            if constexpr (kVec && kElems == 8) {
+                *reinterpret_cast<uint4*>(p + at) = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]),
+                                                               pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+            } else if constexpr (kVec) {
+                *reinterpret_cast<float4*>(p + at) = make_float4(f[0], f[1], f[2], f[3]);
             } else {
 #pragma unroll
-                for (int j = 0; j < 16; ++j)
-                    if (c + j < cols) store_from_float(p + j, f[j]);
+                for (int e = 0; e < kElems; ++e)
+                    if (at + e < left) store_from_float(p + at + e, f[e]);
             }
         }
     }
