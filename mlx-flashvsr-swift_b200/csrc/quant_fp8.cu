@@ -8,9 +8,10 @@
 // flight at once, and keeps in registers. The rows' largest magnitudes are found together: a butterfly in which each step
 // halves the rows a lane still holds (8 shuffles for 16 rows instead of 32), after which a row's code is computed once
 // and handed back with one shuffle. The row form is written from the registers. For the transposed form the tile goes
-// through shared memory once, as stored: a warp then owns 32 rows and a lane two neighbouring columns of them, so that
-// reads are free of bank conflicts and a lane writes 32 consecutive bytes of each of its two lines. Either way x is read
-// once for both forms.
+// through shared memory once, as stored. bf16 comes back through transposing matrix loads whose row addresses are chosen
+// so that a lane receives 16 consecutive rows of one column (16 bytes of its line, four lanes a 64-byte run); a warp owns
+// 16 whole columns, so their maxima need no further exchange. fp32 is read by columns: a warp owns 32 rows, a lane two
+// neighbouring columns of them. Either way x is read once for both forms.
 #include <type_traits>
 
 #include "../../include/fvsr_lcsa.h"
@@ -25,7 +26,7 @@ namespace {
 using namespace sm100;
 
 constexpr int kT = 128, kThreads = 256;
-constexpr uint32_t kAbs = 0x7FFFFFFFu, kAbs2 = 0x7FFF7FFFu;
+constexpr uint32_t kAbs = 0x7FFFFFFFu;
 
 // Elements of T in a 16-byte load, as the pieces of a tile row a lane holds.
 template <typename T>
@@ -37,9 +38,15 @@ struct Piece {
     using Held = std::conditional_t<sizeof(T) == 2, uint2, uint32_t>;  // the piece in 8 bits
 };
 
+__device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b) {  // of |bf16| pairs, NaN above all
+    uint32_t r;
+    asm("{\n\t.reg .b32 t;\n\tabs.bf16x2 t, %2;\n\tmax.NaN.bf16x2 %0, %1, t;\n\t}" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
 // The largest magnitude of a piece, as fp32 bits (an integer maximum: a NaN's bits are above infinity's).
 __device__ __forceinline__ uint32_t piece_max(const uint4& u, const __nv_bfloat16*) {
-    const uint32_t a = __vmaxu2(__vmaxu2(u.x & kAbs2, u.y & kAbs2), __vmaxu2(u.z & kAbs2, u.w & kAbs2));
+    const uint32_t a = max_abs2(max_abs2(max_abs2(max_abs2(0u, u.x), u.y), u.z), u.w);
     return max(a & 0xFFFF0000u, a << 16);
 }
 __device__ __forceinline__ uint32_t piece_max(const uint4& u, const float*) {
@@ -66,6 +73,12 @@ __device__ __forceinline__ void put_piece(uint8_t* p, const uint4& u, uint64_t u
     *reinterpret_cast<uint32_t*>(p) = pack4(fmul2(v.x, up), fmul2(v.y, up));
 }
 
+// Where the 16-byte word `w` of tile row r stands in shared memory. bf16: the words of the eight rows that one matrix
+// load takes (equal but for bits 0, 4 and 5 of the row) lie in different banks.
+template <typename T>
+__device__ __forceinline__ int tile_word(int r, int w) {
+    return r * Piece<T>::kLanes + (sizeof(T) == 2 ? w ^ ((r & 1) | (r >> 3 & 6)) : w);
+}
 // kVec: rows are 16-byte aligned and their lengths whole pieces; else element by element.
 template <typename T, bool kVec>
 __device__ __forceinline__ uint4 load_piece(const T* p, int left) {
@@ -111,7 +124,7 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(int64_t rows, int64_
 #pragma unroll
     for (int i = 0; i < P::kLoads; ++i) {
         top[i] = piece_max(v[i], x);
-        if (kTrans) tile4[(row + i * P::kRowsPerLoad) * P::kLanes + lane % P::kLanes] = v[i];
+        if (kTrans) tile4[tile_word<T>(row + i * P::kRowsPerLoad, lane % P::kLanes)] = v[i];
     }
     // After the butterfly the lanes 2i and 2i + 1 of a row's lanes hold the maximum of load i's row.
 #pragma unroll
@@ -144,25 +157,62 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(int64_t rows, int64_
         const int mine = row + (lane % P::kLanes >> 1) * P::kRowsPerLoad;
         if (!(lane & 1)) put_code(scale, r0 + mine, cb, ct, mine < nr ? code : 0u);
     }
-    if constexpr (kTrans) {
+    if constexpr (kTrans && sizeof(T) == 2) {
+        __syncthreads();
+        const int64_t rt = (rows + kT - 1) / kT, ld = rt * kT;
+        // matrix 4h + m (h = which of a lane's row pairs 0..3 or 4..7, m of one load) has as its row 2j + e tile row
+        // 16j + 2(4h + m) + e, so lane 4·col + j receives rows 16j .. 16j + 15 of its column over the eight matrices
+        const int j2 = lane & 7, m = lane >> 3;
+        const int src_row = 16 * (j2 >> 1) + 2 * m + (j2 & 1);
+#pragma unroll
+        for (int group = 0; group < 2; ++group) {
+            const int w = warp * 2 + group, col = w * 8 + (lane >> 2);  // of the tile
+            uint32_t u[2][8];  // [rows 0..63, 64..127][row pair]
+            uint32_t most2 = 0;
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t* d = u[half] + 4 * h;
+                    const uint32_t at = smem_u32(tile4 + tile_word<T>(64 * half + src_row + 8 * h, w));
+                    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                                 : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+                                 : "r"(at));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) most2 = max_abs2(most2, d[i]);
+                }
+            uint32_t top2 = max(most2 & 0xFFFF0000u, most2 << 16);
+            top2 = max(top2, __shfl_xor_sync(0xffffffffu, top2, 1));
+            top2 = max(top2, __shfl_xor_sync(0xffffffffu, top2, 2));
+            const uint32_t code = fp8_code(square ? most : top2);
+            const float f = fp8_up(code);
+            const uint64_t up = f2(f, f);
+            uint8_t* p = qt + (c0 + col) * ld + r0 + 16 * (lane & 3);
+            if (col < nc) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t o[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        o[i] = pack4(fmul2(bf_pair(u[half][2 * i]), up), fmul2(bf_pair(u[half][2 * i + 1]), up));
+                    *reinterpret_cast<uint4*>(p + 64 * half) = make_uint4(o[0], o[1], o[2], o[3]);
+                }
+            }
+            if ((lane & 3) == 0) put_code(scale_t, c0 + col, rb, rt, col < nc ? code : 0u);
+        }
+    } else if constexpr (kTrans) {
         // lane: columns 2·cp, 2·cp + 1 of the 32 rows [32·quarter, +32)
         __syncthreads();
         const int quarter = warp & 3, cp = (warp >> 2) * 32 + lane;
         const int64_t rt = (rows + kT - 1) / kT, ld = rt * kT;
         const T* tile = reinterpret_cast<const T*>(tile4) + (quarter * 32) * kT + 2 * cp;
         uint32_t ma = 0, mb = 0;
-        uint64_t w[32];  // a row's two columns: a bf16 pair in the low half, or two fp32
+        uint64_t w[32];  // a row's two columns
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-            if constexpr (sizeof(T) == 2) {
-                w[i] = *reinterpret_cast<const uint32_t*>(tile + i * kT);
-                ma = __vmaxu2(ma, (uint32_t)w[i] & kAbs2);
-            } else {
-                w[i] = *reinterpret_cast<const uint64_t*>(tile + i * kT);
-                ma = max(ma, (uint32_t)w[i] & kAbs), mb = max(mb, (uint32_t)(w[i] >> 32) & kAbs);
-            }
+            w[i] = *reinterpret_cast<const uint64_t*>(tile + i * kT);
+            ma = max(ma, (uint32_t)w[i] & kAbs), mb = max(mb, (uint32_t)(w[i] >> 32) & kAbs);
         }
-        if constexpr (sizeof(T) == 2) mb = ma & 0xFFFF0000u, ma <<= 16;
         if (square) {
             ma = mb = most;
         } else {
@@ -181,10 +231,7 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(int64_t rows, int64_
         for (int i = 0; i < 8; ++i) {
             float fa[4], fb[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint64_t p = w[4 * i + j];
-                uf2(fmul2(sizeof(T) == 2 ? bf_pair((uint32_t)p) : p, up), fa[j], fb[j]);
-            }
+            for (int j = 0; j < 4; ++j) uf2(fmul2(w[4 * i + j], up), fa[j], fb[j]);
             a[i] = fp8_pack2(fa[0], fa[1]) | (fp8_pack2(fa[2], fa[3]) << 16);
             b[i] = fp8_pack2(fb[0], fb[1]) | (fp8_pack2(fb[2], fb[3]) << 16);
         }
