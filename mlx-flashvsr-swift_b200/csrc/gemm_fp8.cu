@@ -9,16 +9,26 @@
 // registers, and a weight gradient (a scale for each row and block on both sides) costs what a forward product does.
 //
 // Persistent kernel over CTA pairs (clusters of two CTAs, one TPC): a pair walks 256 × 256 output tiles, CTA r of it
-// loading rows [m0 + 128r, +128) of x and [n0 + 128r, +128) of w per 128-wide K step (32 KB a stage, 6 stages) and, every
-// fourth step, the codes of its 128 rows of x and of all 256 rows of w. Warp roles (320 threads per CTA):
+// loading rows [m0 + 128r, +128) of x and [n0 + 128r, +128) of w per 128-wide K step (32 KB a stage, 4 stages: measured
+// no slower than 5 or 6) and, every fourth step, the codes of its 128 rows of x and of all 256 rows of w. Warp roles (320
+// threads per CTA):
 //   warp 0      TMA producer;
 //   warp 1      TMEM owner and, in the even CTA, the issuer of the scale copies and MMAs (M 256, N 256, K 32);
-//   warps 2..9  epilogue: thread = output row = TMEM lane, each half of the warps 128 of the tile's columns.
+//   warps 2..9  epilogue: thread = output row = TMEM lane, each half of the warps 128 of the tile's columns, 32 at a time
+//               through shared memory in the layout a TMA store takes (16-byte words swizzled, so that the threads'
+//               writes meet no bank conflicts). The residual, where there is one, arrives by TMA in the place the result
+//               is written to. Stores straight from the threads (a row each, 32 rows an instruction) cost 13 % of the
+//               whole product at K = 1536 and remain for rows that are not 16-byte aligned.
 // Tensor memory (512 columns): accumulator 0 in [0, 256), accumulator 1 in [240, 496), the scales in [496, 508). The two
 // accumulators share 16 columns, which an epilogue reads first and releases (ovl) before anything else, so the next
 // tile's MMAs start some hundred cycles into the epilogue and run beside the rest of it.
-// When the tiles are fewer than the pairs, the sum over K is cut into parts (whole tiles of codes, 512 wide) that leave
-// fp32 partial products; a second kernel adds them in order and applies the epilogue.
+//
+// The tensor core adds to its fp32 accumulator by truncation, an error that grows with the number of additions (measured
+// relative to the result: 2e-7 after K = 4096, 1.3e-6 after 17280, on zero-mean operands; a bf16 output does not see it).
+// For an fp32 output the sum is therefore taken in chains of 4096, which the epilogue adds up with rounding, in the
+// output itself: the accumulators alternate between chains as between tiles.
+// When the tiles are fewer than half the pairs, the sum over K is cut into parts (whole tiles of codes, 512 wide) that
+// leave fp32 partial products; a second kernel adds them in order and applies the epilogue.
 // Every wait is bounded (4 s); on expiry the kernel raises its abort and device timeout words, skips the rest of its
 // work and fvsr_device_check reports FVSR_ETIMEOUT.
 #include "../../include/fvsr_lcsa.h"
@@ -34,18 +44,21 @@ namespace {
 
 using namespace sm100;
 
-constexpr int kBM = 256, kBN = 256, kBK = 128, kStages = 6;
+constexpr int kBM = 256, kBN = 256, kBK = 128, kStages = 4;
 constexpr uint32_t kHalfBytes = 128 * kBK;       // 16 KB: one CTA's rows of x or of w per K step
 constexpr uint32_t kStageBytes = 2 * kHalfBytes;
 constexpr uint32_t kScaleBytes = 3 * 512;        // x's 128 rows, w's 256 rows, four blocks
 constexpr int kThreads = 320;
 constexpr int kEpiWarps = 8, kEpiThreads = 32 * kEpiWarps;
+constexpr int kChainBlocks = 32;                 // of 128: the longest chain of an fp32 output
 constexpr uint64_t kWaitLimitNs = 4000000000ull;
 constexpr uint32_t kIdesc = idesc_mxf8(kBM, kBN);
 constexpr uint32_t kAcc1 = 240, kTmemScale = 496;
+constexpr uint32_t kChunkRoom = 8192;            // an epilogue warp's chunks: 4 of 32 × 32 bf16 or 2 of fp32
 constexpr int kBarFull = 0, kBarEmpty = kStages, kBarAccFull = 2 * kStages, kBarAccEmpty = 2 * kStages + 2,
-              kBarOvl = 2 * kStages + 4, kNumBars = 2 * kStages + 5;
-constexpr uint32_t kOffScale = kStages * kStageBytes;
+              kBarOvl = 2 * kStages + 4, kBarSrc = 2 * kStages + 5, kNumBars = kBarSrc + 4 * kEpiWarps;
+constexpr uint32_t kOffChunks = kStages * kStageBytes;
+constexpr uint32_t kOffScale = kOffChunks + kEpiWarps * kChunkRoom;
 constexpr uint32_t kOffBar = kOffScale + kStages * kScaleBytes;
 constexpr uint32_t kOffTmemSlot = kOffBar + 8 * kNumBars;
 constexpr uint32_t kOffAbort = kOffTmemSlot + 4;
@@ -60,62 +73,27 @@ __device__ __forceinline__ float gelu_tanh(float x) {
     return x * rcp_approx(1.0f + ex2_approx(x * fmaf(c1, x * x, c0)));
 }
 
-template <typename T>
-__device__ __forceinline__ float finish(float acc, float bias, float gate, const T* resid, int mode) {
-    float y = acc + bias;
-    if (mode == FVSR_LINEAR_GELU) y = gelu_tanh(y);
-    if (mode == FVSR_LINEAR_GATED_RESIDUAL) y = fmaf(gate, y, load_as_float(resid));
+// What becomes of an accumulator: first / last chain of its sum, add = a value to add (the residual, or what the chains
+// before left).
+template <int kMode>
+__device__ __forceinline__ float finish(float acc, float bias, float gate, float add, bool first, bool last) {
+    float y = first ? acc + bias : acc;
+    if (kMode == FVSR_LINEAR_GATED_RESIDUAL) y *= gate;
+    y += add;
+    if (kMode == FVSR_LINEAR_GELU && last) y = gelu_tanh(y);
     return y;
 }
 
-// 32 consecutive output columns of one row. n = how many of them exist; vec: the row's columns are 16-byte aligned and
-// all there.
-template <typename T, int kMode>
-__device__ __forceinline__ void epilogue_chunk(const uint32_t* v, const float* bias, const float* gate, const T* resid,
-                                               T* out, int n, bool vec) {
-    if (vec) {
-#pragma unroll
-        for (int i = 0; i < 32; i += 8) {
-            float r[8], y[8];
-            if (kMode == FVSR_LINEAR_GATED_RESIDUAL) {
-                if (sizeof(T) == 2) {
-                    const uint4 u = *reinterpret_cast<const uint4*>(resid + i);
-                    bf2_to_f(u.x, r[0], r[1]), bf2_to_f(u.y, r[2], r[3]);
-                    bf2_to_f(u.z, r[4], r[5]), bf2_to_f(u.w, r[6], r[7]);
-                } else {
-                    *reinterpret_cast<float4*>(r) = *reinterpret_cast<const float4*>(resid + i);
-                    *reinterpret_cast<float4*>(r + 4) = *reinterpret_cast<const float4*>(resid + i + 4);
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                y[j] = __uint_as_float(v[i + j]) + bias[i + j];
-                if (kMode == FVSR_LINEAR_GELU) y[j] = gelu_tanh(y[j]);
-                if (kMode == FVSR_LINEAR_GATED_RESIDUAL) y[j] = fmaf(gate[i + j], y[j], r[j]);
-            }
-            if (sizeof(T) == 2) {
-                *reinterpret_cast<uint4*>(out + i) = make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]),
-                                                                pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7]));
-            } else {
-                *reinterpret_cast<float4*>(out + i) = make_float4(y[0], y[1], y[2], y[3]);
-                *reinterpret_cast<float4*>(out + i + 4) = make_float4(y[4], y[5], y[6], y[7]);
-            }
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-            if (i < n) store_from_float(out + i, finish(__uint_as_float(v[i]), bias[i], gate[i], resid + i, kMode));
-    }
-}
-
 struct Work {
-    int mt, nt, kt, splits, part_blocks;
+    int mt, nt, kt, splits, part_blocks, chain_blocks;
+    int tma;  // rows of out (and resid) are 16-byte aligned
 };
 
 template <typename T, int kMode>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     gemm_fp8_sm100_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
                           const __grid_constant__ CUtensorMap tmXS, const __grid_constant__ CUtensorMap tmWS,
+                          const __grid_constant__ CUtensorMap tmOut, const __grid_constant__ CUtensorMap tmResid,
                           const Fp8GemmArgs a, const Work wk) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -146,6 +124,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             mbar_init(bar(kBarAccEmpty + b), 2 * kEpiWarps);
         }
         mbar_init(bar(kBarOvl), kEpiWarps);
+        for (int b = 0; b < 4 * kEpiWarps; ++b) mbar_init(bar(kBarSrc + b), 1);
         *abort_word = 0;
         fence_mbar_init();
     }
@@ -154,6 +133,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         prefetch_tmap(&tmW);
         prefetch_tmap(&tmXS);
         prefetch_tmap(&tmWS);
+        prefetch_tmap(&tmOut);
     }
     griddep_wait_then_release();
     if (warp == 1) {
@@ -200,38 +180,40 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             uint32_t it = 0;
             bool ok = true;
             int lt = 0;
-            for (int t = pair; ok && t < items; t += npairs, ++lt) {
+            for (int t = pair; ok && t < items; t += npairs) {
                 int m0, n0, kb0, kb1;
                 place(t, m0, n0, kb0, kb1);
-                const int acc = lt & 1;
-                if (lt >= 2 && !(ok = wait(kBarAccEmpty + acc, (uint32_t)((lt >> 1) - 1)))) break;
-                if (lt >= 1 && !(ok = wait(kBarOvl, (uint32_t)(lt - 1)))) break;
-                tc_fence_after();
-                const uint32_t d = tmem + (acc ? kAcc1 : 0u), sf = tmem + kTmemScale;
-                for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                    const int st = (int)(it % kStages);
-                    if (!(ok = wait(kBarFull + st, it / kStages))) break;
+                for (int cb = kb0; ok && cb < kb1; cb += wk.chain_blocks, ++lt) {
+                    const int acc = lt & 1, ce = min(cb + wk.chain_blocks, kb1);
+                    if (lt >= 2 && !(ok = wait(kBarAccEmpty + acc, (uint32_t)((lt >> 1) - 1)))) break;
+                    if (lt >= 1 && !(ok = wait(kBarOvl, (uint32_t)(lt - 1)))) break;
                     tc_fence_after();
-                    const uint32_t sa = sbase + (uint32_t)st * kStageBytes;
-                    if ((kb & 3) == 0) {
-                        const uint32_t sc = sbase + kOffScale + (uint32_t)st * kScaleBytes;
-                        tmem_cp_scales_pair(sf, scale_desc(sc));
-                        tmem_cp_scales_pair(sf + 4, scale_desc(sc + 512));
-                        tmem_cp_scales_pair(sf + 8, scale_desc(sc + 1024));
-                    }
-                    const uint64_t ad = smem_desc(sa, 16, 1024);
-                    const uint64_t bd = smem_desc(sa + kHalfBytes, 16, 1024);
-                    const uint32_t idesc = kIdesc | idesc_sf_id((uint32_t)kb & 3u);
+                    const uint32_t d = tmem + (acc ? kAcc1 : 0u), sf = tmem + kTmemScale;
+                    for (int kb = cb; kb < ce; ++kb, ++it) {
+                        const int st = (int)(it % kStages);
+                        if (!(ok = wait(kBarFull + st, it / kStages))) break;
+                        tc_fence_after();
+                        const uint32_t sa = sbase + (uint32_t)st * kStageBytes;
+                        if ((kb & 3) == 0) {
+                            const uint32_t sc = sbase + kOffScale + (uint32_t)st * kScaleBytes;
+                            tmem_cp_scales_pair(sf, scale_desc(sc));
+                            tmem_cp_scales_pair(sf + 4, scale_desc(sc + 512));
+                            tmem_cp_scales_pair(sf + 8, scale_desc(sc + 1024));
+                        }
+                        const uint64_t ad = smem_desc(sa, 16, 1024);
+                        const uint64_t bd = smem_desc(sa + kHalfBytes, 16, 1024);
+                        const uint32_t idesc = kIdesc | idesc_sf_id((uint32_t)kb & 3u);
 #pragma unroll
-                    for (int kk = 0; kk < kBK / 32; ++kk)
-                        mma_mxf8_pair(d, ad + (uint64_t)(2 * kk), bd + (uint64_t)(2 * kk), idesc, sf, sf + 4,
-                                      (kb > kb0 || kk > 0) ? 1u : 0u);
-                    mma_commit_pair(bar(kBarEmpty + st));
-                    mma_commit_pair(mapa_shared(bar(kBarEmpty + st), 1));
-                }
-                if (ok) {
-                    mma_commit_pair(bar(kBarAccFull + acc));
-                    mma_commit_pair(mapa_shared(bar(kBarAccFull + acc), 1));
+                        for (int kk = 0; kk < kBK / 32; ++kk)
+                            mma_mxf8_pair(d, ad + (uint64_t)(2 * kk), bd + (uint64_t)(2 * kk), idesc, sf, sf + 4,
+                                          (kb > cb || kk > 0) ? 1u : 0u);
+                        mma_commit_pair(bar(kBarEmpty + st));
+                        mma_commit_pair(mapa_shared(bar(kBarEmpty + st), 1));
+                    }
+                    if (ok) {
+                        mma_commit_pair(bar(kBarAccFull + acc));
+                        mma_commit_pair(mapa_shared(bar(kBarAccFull + acc), 1));
+                    }
                 }
             }
         }
@@ -244,57 +226,147 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         float* bias_s = reinterpret_cast<float*>(smem + kOffCols);
         float* gate_s = bias_s + kBN;
         const uint32_t acc_empty0 = mapa_shared(bar(kBarAccEmpty), 0), ovl0 = mapa_shared(bar(kBarOvl), 0);
-        const bool aligned_rows = ((int64_t)a.N * sizeof(T)) % 16 == 0 &&
-                                  ((reinterpret_cast<uintptr_t>(a.out) | reinterpret_cast<uintptr_t>(a.resid)) & 15) == 0;
+        constexpr bool kBf16 = sizeof(T) == 2;
+        constexpr int kRoom = kBf16 ? 4 : 2;  // chunks in flight
+        constexpr uint32_t kRowBytes = 32 * sizeof(T), kChunkBytes = 32 * kRowBytes;
+        uint8_t* const chunks = smem + kOffChunks + (uint32_t)(warp - 2) * kChunkRoom;
+        const uint32_t swizzle = (kBf16 ? (uint32_t)lane >> 1 & 3u : (uint32_t)lane & 7u) << 4;
+        const int src_bar = kBarSrc + 4 * (warp - 2);
+        uint32_t src_phase = 0;  // bit b: parity of the next wait on chunk place b
         int lt = 0;
         bool ok = true;
-        for (int t = pair; t < items; t += npairs, ++lt) {
+        for (int t = pair; t < items; t += npairs) {
             int m0, n0, kb0, kb1;
             place(t, m0, n0, kb0, kb1);
-            const int acc = lt & 1;
             named_barrier_sync(1, kEpiThreads);
             bias_s[et] = a.bias && n0 + et < a.N ? __bfloat162float(a.bias[n0 + et]) : 0.0f;
             gate_s[et] = kMode == FVSR_LINEAR_GATED_RESIDUAL && n0 + et < a.N ? __bfloat162float(a.gate[n0 + et]) : 0.0f;
             named_barrier_sync(1, kEpiThreads);
-            const int64_t row = (int64_t)m0 + 128 * (int)rank + r;
+            const int row0 = m0 + 128 * (int)rank + quarter * 32, plane = t % wk.splits;
             const int c0 = n0 + half * (kBN / 2);
-            const int64_t at = (wk.splits > 1 ? (int64_t)(t % wk.splits) * a.M * a.N : 0) + row * a.N + c0;
-            if (ok) ok = __all_sync(0xffffffffu, wait(kBarAccFull + acc, (uint32_t)(lt >> 1)));
-            if (!ok) continue;
-            tc_fence_after();
-            T* orow = static_cast<T*>(a.out) + at;
-            const T* rrow = static_cast<const T*>(a.resid) + at;
             const float *bcol = bias_s + half * (kBN / 2), *gcol = gate_s + half * (kBN / 2);
-            const uint32_t tbase = lane_base + (acc ? kAcc1 : 0u);
-            // accumulator 0 from its last chunk to its first, accumulator 1 from its first: the shared columns come first
-            auto chunk = [&](int i) { return acc ? i : kBN / 64 - 1 - i; };
-            auto emit = [&](const uint32_t* v, int c) {
-                const int left = a.N - (c0 + 32 * c);
-                if (row < a.M && left > 0)
-                    epilogue_chunk<T, kMode>(v, bcol + 32 * c, gcol + 32 * c, rrow + 32 * c, orow + 32 * c, left,
-                                             aligned_rows && left >= 32);
-            };
-            uint32_t va[32], vb[32];
-            tmem_ld32(tbase + 32u * (uint32_t)chunk(0), va);
-            tmem_ld_wait(va);
-            if (half != acc) {  // this half held the shared columns: half 1 of accumulator 0, half 0 of accumulator 1
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(ovl0);
-            }
+            for (int cb = kb0; cb < kb1; cb += wk.chain_blocks, ++lt) {
+                const int acc = lt & 1;
+                const bool first = cb == kb0, last = cb + wk.chain_blocks >= kb1;
+                const bool src = !first || kMode == FVSR_LINEAR_GATED_RESIDUAL;  // something to add: chains before, resid
+                // accumulator 0 from its last chunk to its first, accumulator 1 from its first: the shared columns come first
+                auto chunk = [&](int i) { return acc ? i : kBN / 64 - 1 - i; };
+                auto live = [&](int c) { return row0 < a.M && c0 + 32 * c < a.N; };
+                auto fetch = [&](int i) {  // by lane 0: the values to add to chunk i into its place
+                    const int c = chunk(i);
+                    if (!live(c)) return;
+                    const uint32_t b = bar(src_bar + i % kRoom);
+                    mbar_expect_tx(b, kChunkBytes);
+                    tma_load_3d(smem_u32(chunks + (i % kRoom) * kChunkBytes), first ? &tmResid : &tmOut, c0 + 32 * c,
+                                row0, plane, b);
+                };
+                if (wk.tma && src && ok && lane == 0) {
+                    if (first) bulk_wait_read<0>();
+                    else bulk_wait<0>();  // the chain before is in memory
+                    for (int i = 0; i < kRoom; ++i) fetch(i);
+                }
+                if (ok) ok = __all_sync(0xffffffffu, wait(kBarAccFull + acc, (uint32_t)(lt >> 1)));
+                if (!ok) continue;
+                tc_fence_after();
+                const uint32_t tbase = lane_base + (acc ? kAcc1 : 0u);
+                auto emit = [&](const uint32_t* v, int i) {
+                    const int c = chunk(i);
+                    const float *bias = bcol + 32 * c, *gate = gcol + 32 * c;
+                    auto fetch_next = [&] {  // by lane 0, once this chunk's place is free again
+                        if (src && i + kRoom < kBN / 64) {
+                            bulk_wait_read<0>();
+                            fetch(i + kRoom);
+                        }
+                    };
+                    if (!live(c)) {
+                        if (wk.tma && lane == 0) {
+                            bulk_commit();  // keeps the groups' count
+                            fetch_next();
+                        }
+                        return;
+                    }
+                    if (wk.tma) {
+                        const int place_i = i % kRoom;
+                        uint8_t* mine = chunks + place_i * kChunkBytes + (uint32_t)lane * kRowBytes;
+                        if (src) {
+                            const bool here = wait(src_bar + place_i, src_phase >> place_i);
+                            src_phase ^= 1u << place_i;
+                            if (!__all_sync(0xffffffffu, here)) ok = false;
+                        } else {
+                            if (lane == 0) bulk_wait_read<kRoom - 1>();
+                            __syncwarp();
+                        }
+                        constexpr int kWord = 16 / sizeof(T);
 #pragma unroll
-            for (int i = 0; i < kBN / 64; i += 2) {
-                tmem_ld32(tbase + 32u * (uint32_t)chunk(i + 1), vb);
-                emit(va, chunk(i));
-                tmem_ld_wait(vb);
-                if (i + 2 < kBN / 64) tmem_ld32(tbase + 32u * (uint32_t)chunk(i + 2), va);
-                emit(vb, chunk(i + 1));
-                if (i + 2 < kBN / 64) tmem_ld_wait(va);
+                        for (int w = 0; w < 32 / kWord; ++w) {
+                            uint4* at = reinterpret_cast<uint4*>(mine + (((uint32_t)w << 4) ^ swizzle));
+                            float add[kWord] = {}, y[kWord];
+                            if (src) {
+                                const uint4 u = *at;
+                                if constexpr (kBf16) {
+                                    bf2_to_f(u.x, add[0], add[1]), bf2_to_f(u.y, add[2], add[3]);
+                                    bf2_to_f(u.z, add[4], add[5]), bf2_to_f(u.w, add[6], add[7]);
+                                } else {
+                                    add[0] = __uint_as_float(u.x), add[1] = __uint_as_float(u.y);
+                                    add[2] = __uint_as_float(u.z), add[3] = __uint_as_float(u.w);
+                                }
+                            }
+#pragma unroll
+                            for (int e = 0; e < kWord; ++e)
+                                y[e] = finish<kMode>(__uint_as_float(v[w * kWord + e]), bias[w * kWord + e],
+                                                     gate[w * kWord + e], add[e], kBf16 || first, kBf16 || last);
+                            if constexpr (kBf16)
+                                *at = make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]),
+                                                 pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7]));
+                            else
+                                *at = make_uint4(__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]),
+                                                 __float_as_uint(y[3]));
+                        }
+                        fence_async_shared();
+                        __syncwarp();
+                        if (lane == 0) {
+                            tma_store_3d(&tmOut, c0 + 32 * c, row0, plane, smem_u32(mine));
+                            bulk_commit();
+                            fetch_next();
+                        }
+                    } else if (row0 + lane < a.M) {
+                        const int64_t at = (int64_t)(row0 + lane) * a.N + c0 + 32 * c;
+                        T* out = static_cast<T*>(a.out) + at;
+                        const T* from = first ? static_cast<const T*>(a.resid) + at : out;
+                        const int left = a.N - (c0 + 32 * c);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (e < left)
+                                store_from_float(out + e, finish<kMode>(__uint_as_float(v[e]), bias[e], gate[e],
+                                                                        src ? load_as_float(from + e) : 0.0f,
+                                                                        kBf16 || first, kBf16 || last));
+                    }
+                };
+                uint32_t va[32], vb[32];
+                tmem_ld32(tbase + 32u * (uint32_t)chunk(0), va);
+                tmem_ld_wait(va);
+                if (half != acc) {  // this half held the shared columns: half 1 of accumulator 0, half 0 of accumulator 1
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(ovl0);
+                }
+#pragma unroll
+                for (int i = 0; i < kBN / 64; i += 2) {
+                    tmem_ld32(tbase + 32u * (uint32_t)chunk(i + 1), vb);
+                    emit(va, i);
+                    tmem_ld_wait(vb);
+                    if (i + 2 < kBN / 64) tmem_ld32(tbase + 32u * (uint32_t)chunk(i + 2), va);
+                    if (i + 2 == kBN / 64) {  // the accumulator is in registers
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_cluster(acc_empty0 + 8u * (uint32_t)acc);
+                    }
+                    emit(vb, i + 1);
+                    if (i + 2 < kBN / 64) tmem_ld_wait(va);
+                }
             }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(acc_empty0 + 8u * (uint32_t)acc);
         }
+        if (wk.tma && lane == 0) bulk_wait<0>();
     }
     tc_fence_before();
     cluster_sync();  // no signal to the other CTA and no MMA on this CTA's shared memory is still in flight
@@ -304,45 +376,74 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
 }
 
-// out = epilogue(Σ partial products in order + bias), one thread per element.
-template <typename T>
+// out = epilogue(Σ partial products in order + bias), a thread four columns of a row.
+template <typename T, int kMode>
 __global__ void __launch_bounds__(256) gemm_fp8_join_kernel(const Fp8GemmArgs a, const float* __restrict__ partial,
-                                                            int splits) {
+                                                            int splits, int64_t ld) {
     griddep_wait_then_release();
-    const int64_t n = (int64_t)a.M * a.N;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        float s = partial[i];
-        for (int p = 1; p < splits; ++p) s += partial[p * n + i];
-        const int c = (int)(i % a.N);
-        store_from_float(static_cast<T*>(a.out) + i,
-                         finish(s, a.bias ? __bfloat162float(a.bias[c]) : 0.0f,
-                                a.gate ? __bfloat162float(a.gate[c]) : 0.0f, static_cast<const T*>(a.resid) + i, a.mode));
+    const int quads = (int)(ld >> 2);
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / quads;
+    if (row >= a.M) return;
+    const int col = (int)(i % quads) * 4, left = min(4, a.N - col);
+    const int64_t plane = (int64_t)a.M * ld;
+    const float* p = partial + row * ld + col;
+    float4 s = *reinterpret_cast<const float4*>(p);
+#pragma unroll 4
+    for (int k = 1; k < splits; ++k) {
+        const float4 v = *reinterpret_cast<const float4*>(p + k * plane);
+        s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
     }
+    const float v[4] = {s.x, s.y, s.z, s.w};
+    T* out = static_cast<T*>(a.out) + row * a.N + col;
+    const T* resid = static_cast<const T*>(a.resid) + row * a.N + col;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (e < left)
+            store_from_float(out + e,
+                             finish<kMode>(v[e], a.bias ? __bfloat162float(a.bias[col + e]) : 0.0f,
+                                           kMode == FVSR_LINEAR_GATED_RESIDUAL ? __bfloat162float(a.gate[col + e]) : 0.0f,
+                                           kMode == FVSR_LINEAR_GATED_RESIDUAL ? load_as_float(resid + e) : 0.0f, true, true));
 }
 
+struct Maps {
+    CUtensorMap x, w, xs, ws, out, resid;
+};
+
 template <typename T, int kMode>
-cudaError_t launch_tiles(const Fp8GemmArgs& args, const Work& wk, const CUtensorMap (&maps)[4], cudaStream_t st) {
+cudaError_t launch_tiles(const Fp8GemmArgs& args, const Work& wk, const Maps& m, cudaStream_t st) {
     auto kernel = gemm_fp8_sm100_kernel<T, kMode>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes);
     if (e != cudaSuccess) return e;
     const int items = wk.mt * wk.nt * wk.splits, pairs = sm_count() / 2;
-    return launch_pdl(kernel, dim3(2 * (items < pairs ? items : pairs)), dim3(kThreads), kSmemBytes, st, maps[0],
-                      maps[1], maps[2], maps[3], args, wk);
+    return launch_pdl(kernel, dim3(2 * (items < pairs ? items : pairs)), dim3(kThreads), kSmemBytes, st, m.x, m.w, m.xs,
+                      m.ws, m.out, m.resid, args, wk);
 }
 
 template <typename T>
-cudaError_t launch_mode(const Fp8GemmArgs& args, const Work& wk, const CUtensorMap (&maps)[4], cudaStream_t st) {
+cudaError_t launch_mode(const Fp8GemmArgs& args, const Work& wk, const Maps& m, cudaStream_t st) {
     switch (args.mode) {
-        case FVSR_LINEAR: return launch_tiles<T, FVSR_LINEAR>(args, wk, maps, st);
-        case FVSR_LINEAR_GELU: return launch_tiles<T, FVSR_LINEAR_GELU>(args, wk, maps, st);
-        default: return launch_tiles<T, FVSR_LINEAR_GATED_RESIDUAL>(args, wk, maps, st);
+        case FVSR_LINEAR: return launch_tiles<T, FVSR_LINEAR>(args, wk, m, st);
+        case FVSR_LINEAR_GELU: return launch_tiles<T, FVSR_LINEAR_GELU>(args, wk, m, st);
+        default: return launch_tiles<T, FVSR_LINEAR_GATED_RESIDUAL>(args, wk, m, st);
     }
 }
+
+template <typename T>
+cudaError_t launch_join(const Fp8GemmArgs& a, const Fp8GemmPlan& p, const float* partial, cudaStream_t st) {
+    const dim3 grid((unsigned)(((int64_t)a.M * (p.partial_ld >> 2) + 255) / 256)), block(256);
+    switch (a.mode) {
+        case FVSR_LINEAR: return launch_pdl(gemm_fp8_join_kernel<T, FVSR_LINEAR>, grid, block, 0, st, a, partial, p.splits, p.partial_ld);
+        case FVSR_LINEAR_GELU: return launch_pdl(gemm_fp8_join_kernel<T, FVSR_LINEAR_GELU>, grid, block, 0, st, a, partial, p.splits, p.partial_ld);
+        default: return launch_pdl(gemm_fp8_join_kernel<T, FVSR_LINEAR_GATED_RESIDUAL>, grid, block, 0, st, a, partial, p.splits, p.partial_ld);
+    }
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 }  // namespace
 
 Fp8GemmPlan plan_gemm_fp8(int M, int N, int K) {
-    Fp8GemmPlan p{1, 0, 0};
+    Fp8GemmPlan p{1, 0, 0, 0};
     const int kt = (K + kBK - 1) / kBK, groups = (kt + 3) / 4;
     const int64_t tiles = (int64_t)((M + kBM - 1) / kBM) * ((N + kBN - 1) / kBN);
     const int pairs = sm_count() / 2;
@@ -351,39 +452,43 @@ Fp8GemmPlan plan_gemm_fp8(int M, int N, int K) {
     const int per = (groups + splits - 1) / splits;
     p.splits = (groups + per - 1) / per;
     p.part_blocks = 4 * per;
-    if (p.splits > 1) p.partial_bytes = (size_t)p.splits * M * N * sizeof(float);
+    if (p.splits > 1) {
+        p.partial_ld = (N + 3) / 4 * 4;  // 16-byte rows
+        p.partial_bytes = (size_t)p.splits * M * p.partial_ld * sizeof(float);
+    }
     return p;
 }
 
 cudaError_t launch_gemm_fp8(const Fp8GemmArgs& args, const Fp8GemmPlan& plan, float* partial, cudaStream_t st) {
+    const bool parts = plan.splits > 1, bf16 = args.out_dtype == FVSR_BF16;
     Work wk;
     wk.mt = (args.M + kBM - 1) / kBM;
     wk.nt = (args.N + kBN - 1) / kBN;
     wk.kt = (args.K + kBK - 1) / kBK;
     wk.splits = plan.splits;
     wk.part_blocks = plan.part_blocks;
-    CUtensorMap maps[4];
+    wk.chain_blocks = bf16 ? plan.part_blocks : kChainBlocks;
+    const bool gated = args.mode == FVSR_LINEAR_GATED_RESIDUAL;
+    wk.tma = parts || ((int64_t)args.N * (bf16 ? 2 : 4) % 16 == 0 && aligned16(args.out) && (!gated || aligned16(args.resid)));
+    Maps m;
     const int64_t ld = fp8_ld(args.K), kt4 = fp8_scale_tiles(args.K);
-    if (!make_byte_map(&maps[0], args.x, args.M, ld, 128) || !make_byte_map(&maps[1], args.w, args.N, ld, 128) ||
-        !make_scale_map(&maps[2], args.x_scale, ((int64_t)args.M + 127) / 128 * kt4) ||
-        !make_scale_map(&maps[3], args.w_scale, ((int64_t)args.N + 127) / 128 * kt4))
-        return cudaErrorInvalidValue;
-    if (plan.splits == 1)
-        return args.out_dtype == FVSR_BF16 ? launch_mode<__nv_bfloat16>(args, wk, maps, st)
-                                           : launch_mode<float>(args, wk, maps, st);
-    Fp8GemmArgs parts = args;
-    parts.out = partial;
-    parts.bias = nullptr;
-    parts.mode = FVSR_LINEAR;
-    parts.resid = nullptr;
-    cudaError_t e = launch_tiles<float, FVSR_LINEAR>(parts, wk, maps, st);
+    bool made = make_byte_map(&m.x, args.x, args.M, ld, 128) && make_byte_map(&m.w, args.w, args.N, ld, 128) &&
+                make_scale_map(&m.xs, args.x_scale, ((int64_t)args.M + 127) / 128 * kt4) &&
+                make_scale_map(&m.ws, args.w_scale, ((int64_t)args.N + 127) / 128 * kt4);
+    m.out = m.resid = m.x;  // not used without tma
+    if (parts)
+        made = made && make_chunk_map(&m.out, partial, false, plan.splits, args.M, args.N, plan.partial_ld);
+    else if (wk.tma)
+        made = made && make_chunk_map(&m.out, args.out, bf16, 1, args.M, args.N, args.N) &&
+               (!gated || make_chunk_map(&m.resid, args.resid, bf16, 1, args.M, args.N, args.N));
+    if (!made) return cudaErrorInvalidValue;
+    if (!parts) return bf16 ? launch_mode<__nv_bfloat16>(args, wk, m, st) : launch_mode<float>(args, wk, m, st);
+    Fp8GemmArgs sums = args;
+    sums.bias = nullptr;
+    sums.mode = FVSR_LINEAR;
+    cudaError_t e = launch_tiles<float, FVSR_LINEAR>(sums, wk, m, st);
     if (e != cudaSuccess) return e;
-    const int64_t blocks = ((int64_t)args.M * args.N + 255) / 256, most = (int64_t)sm_count() * 8;
-    const dim3 grid((unsigned)(blocks < most ? blocks : most));
-    return args.out_dtype == FVSR_BF16
-               ? launch_pdl(gemm_fp8_join_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, args, (const float*)partial,
-                            plan.splits)
-               : launch_pdl(gemm_fp8_join_kernel<float>, grid, dim3(256), 0, st, args, (const float*)partial, plan.splits);
+    return bf16 ? launch_join<__nv_bfloat16>(args, plan, partial, st) : launch_join<float>(args, plan, partial, st);
 }
 
 cudaError_t read_and_clear_gemm_fp8_error(int* flag) {
