@@ -773,7 +773,7 @@ def _elsewhere(t, stream):
         if stream.device != t.device:
             raise FVSRError(FVSR_EINVAL, f"the stream is on {stream.device}, the tensors on {t.device}")
         return torch.cuda.stream(stream)
-    if torch.cuda.current_device() != t.get_device():
+    if torch._C._cuda_getDevice() != t.get_device():
         return torch.cuda.device(t.get_device())
     return None
 
@@ -801,7 +801,8 @@ def _channel_vector(t, name, n, dtype, like):
     """The address of a contiguous (n,) tensor of dtype on like's device (None: no such vector), or FVSRError."""
     if t is None:
         return None
-    if t.dtype != dtype or t.shape != (n,) or t.get_device() != like.get_device() or not t.is_contiguous():
+    if t.dtype != dtype or t.dim() != 1 or t.numel() != n or t.get_device() != like.get_device() or \
+            not t.is_contiguous():
         raise FVSRError(FVSR_EINVAL, f"{name} must be contiguous ({n},) {dtype} on {like.device}")
     return t.data_ptr()
 
@@ -917,7 +918,9 @@ def linear_fp8(x, w: Fp8Tensor, bias=None, epilogue: int = FVSR_LINEAR, gate=Non
         raise FVSRError(FVSR_EINVAL, f"out must be bfloat16 or float32 as out_dtype says, got {out_dtype}")
     if resid is not None:
         resid = _matrix(resid, "resid", dtypes=(out.dtype,), shape=(m, n), like=xt).data_ptr()
-    need = linear_fp8_workspace_size(m, n, k, held) if workspace is None else 0
+    need = 0
+    if workspace is None:
+        need = _bytes("fvsr_linear_fp8_workspace_size", xt.get_device(), m, n, k, 1 if held else 0)
     ws, ws_bytes, workspace = _scratch(workspace, need, xt)
     _check(lib().fvsr_linear_fp8(m, n, k, xt.data_ptr(), x.scale.data_ptr() if held else None, w.data.data_ptr(),
                                  w.scale.data_ptr(), bias, epilogue, gate, resid, out.data_ptr(), _dtype_code(out), ws,
@@ -927,8 +930,9 @@ def linear_fp8(x, w: Fp8Tensor, bias=None, epilogue: int = FVSR_LINEAR, gate=Non
 
 def linear_fp8_workspace_size(m: int, n: int, k: int, x_is_fp8: bool) -> int:
     """Bytes of workspace of a linear_fp8 call on the current device."""
-    device = _torch().cuda.current_device() if _torch().cuda.is_available() else -1
-    return _bytes("fvsr_linear_fp8_workspace_size", device, m, n, k, 1 if x_is_fp8 else 0)
+    cuda = _torch().cuda
+    return _bytes("fvsr_linear_fp8_workspace_size", cuda.current_device() if cuda.is_available() else -1, m, n, k,
+                  1 if x_is_fp8 else 0)
 
 
 def layernorm_train(x, weight=None, bias=None, shift=None, scale=None, eps: float = 1e-6, out=None, stream=None):

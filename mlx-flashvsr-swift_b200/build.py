@@ -20,7 +20,8 @@ OUT_DIR = PKG / "_build"
 LIB = PKG / "libfvsr_lcsa.so"
 SOURCES = ["pool.cu", "prepare.cu", "select.cu", "attn_f32.cu", "attn_sm100.cu", "attn_persist.cu", "schedule.cu",
            "api.cu", "stream.cu", "select_noalloc.cu", "gemm.cu", "norm.cu",
-           "api_fp8.cu", "quant_fp8.cu", "gemm_fp8.cu", "norm_train.cu"]
+           "api_fp8.cu", "quant_fp8.cu", "gemm_fp8.cu", "gemv_fp8.cu",
+           "norm_train.cu"]
 
 
 def nvcc() -> str:

@@ -141,7 +141,7 @@ fvsr_status fvsr_linear_fp8_workspace_size(int32_t m, int32_t n, int32_t k, int3
     fvsr_status s = check_linear_shape(m, n, k);
     if (s != FVSR_OK) return s;
     if (!bytes) return refuse(FVSR_EINVAL, "bytes is NULL");
-    *bytes = m == 0 ? 0 : linear_workspace(m, n, k, x_is_fp8 != 0).bytes;
+    *bytes = m <= kFewTokens ? 0 : linear_workspace(m, n, k, x_is_fp8 != 0).bytes;
     return FVSR_OK;
 }
 
@@ -160,7 +160,8 @@ fvsr_status fvsr_linear_fp8(int32_t m, int32_t n, int32_t k, const void* x, cons
     if (!aligned(x, 16) || !aligned(x_scale, 16) || !aligned(w, 16) || !aligned(w_scale, 16) || !aligned(out, 4) ||
         !aligned(resid, 4) || !aligned(bias, 2) || !aligned(gate, 2))
         return refuse(FVSR_EINVAL, "x, w and the scales must be 16-byte aligned, out and resid 4-byte, bias and gate 2-byte aligned");
-    const LinearWorkspace ws = linear_workspace(m, n, k, x_scale != nullptr);
+    const bool few = m <= kFewTokens;
+    const LinearWorkspace ws = few ? LinearWorkspace{} : linear_workspace(m, n, k, x_scale != nullptr);
     const size_t need = ws.bytes;
     if (need > 0 && !workspace) return refuse(FVSR_EINVAL, "the workspace is required");
     if (workspace_bytes < need)
@@ -172,7 +173,7 @@ fvsr_status fvsr_linear_fp8(int32_t m, int32_t n, int32_t k, const void* x, cons
     a.M = m, a.N = n, a.K = k;
     a.x = static_cast<const uint8_t*>(x);
     a.x_scale = static_cast<const uint8_t*>(x_scale);
-    if (!x_scale) {
+    if (!x_scale && !few) {
         uint8_t* q = static_cast<uint8_t*>(workspace);
         uint8_t* scale = q + ws.scale;
         s = launched(launch_quantize_fp8(m, k, x, FVSR_BF16, false, q, scale, nullptr, nullptr, st), "quantize launch");
@@ -187,6 +188,8 @@ fvsr_status fvsr_linear_fp8(int32_t m, int32_t n, int32_t k, const void* x, cons
     a.out = out;
     a.mode = epilogue;
     a.out_dtype = out_dtype;
+    if (few)
+        return launched(launch_gemv_fp8(a, x_scale ? nullptr : static_cast<const __nv_bfloat16*>(x), st), "linear launch");
     return launched(launch_gemm_fp8(a, ws.plan, reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ws.partial),
                                     st), "linear launch");
 }

@@ -13,6 +13,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace fvsr {
 
 __host__ __device__ inline int64_t fp8_ld(int64_t cols) { return (cols + 127) / 128 * 128; }
@@ -60,12 +62,28 @@ __device__ __forceinline__ float load_as_float(const __nv_bfloat16* p) { return 
 __device__ __forceinline__ void store_from_float(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_from_float(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-// Multiprocessors of the current device.
+// Multiprocessors of the current device (asked for once per device).
 inline int sm_count() {
+    static std::atomic<int> known[64];
     int dev = 0, n = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-        return 148;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+    if (dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+    if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
     return n;
+}
+// Lets `kernel` take `bytes` of dynamic shared memory on the current device (once per kernel and device: kernel is a
+// template argument so that each has its own record).
+template <auto kernel>
+cudaError_t allow_smem(size_t bytes) {
+    static std::atomic<int> allowed[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 64 && (size_t)allowed[dev].load(std::memory_order_relaxed) >= bytes) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess && dev < 64) allowed[dev].store((int)bytes, std::memory_order_relaxed);
+    return e;
 }
 
 // ---- launchers ----
@@ -77,7 +95,7 @@ cudaError_t launch_fp8_codes(int64_t rows, int64_t cols, const uint8_t* scale, u
 cudaError_t launch_dequantize_fp8(int64_t rows, int64_t cols, const uint8_t* q, const uint8_t* scale, void* out,
                                   int dtype, cudaStream_t st);
 
-// out (M, N) = epilogue(x · wᵀ + bias) on 8-bit operands (gemm_fp8.cu).
+// out (M, N) = epilogue(x · wᵀ + bias) on 8-bit operands (gemm_fp8.cu, gemv_fp8.cu).
 struct Fp8GemmArgs {
     int M, N, K;
     const uint8_t* x;         // (M, ld(K)) e4m3
@@ -98,6 +116,9 @@ struct Fp8GemmPlan {
     size_t partial_bytes;
 };
 Fp8GemmPlan plan_gemm_fp8(int M, int N, int K);
+// Up to kFewTokens rows of x, without a workspace: x in a.x / a.x_scale, or bf16 in xb (gemv_fp8.cu).
+constexpr int kFewTokens = 16;
+cudaError_t launch_gemv_fp8(const Fp8GemmArgs& a, const __nv_bfloat16* xb, cudaStream_t st);
 cudaError_t launch_gemm_fp8(const Fp8GemmArgs& a, const Fp8GemmPlan& plan, float* partial, cudaStream_t st);
 
 // LayerNorm for training (norm_train.cu).

@@ -17,8 +17,11 @@
 //   warps 2..9  epilogue: thread = output row = TMEM lane, each half of the warps 128 of the tile's columns, 32 at a time
 //               through shared memory in the layout a TMA store takes (16-byte words swizzled, so that the threads'
 //               writes meet no bank conflicts). The residual, where there is one, arrives by TMA in the place the result
-//               is written to. Stores straight from the threads (a row each, 32 rows an instruction) cost 13 % of the
-//               whole product at K = 1536 and remain for rows that are not 16-byte aligned.
+//               is written to. (Stores straight from the threads, a row each and 32 rows an instruction, cost 13 % of
+//               the whole product at K = 1536.) Rows that are not 16-byte aligned take the same way through shared
+//               memory and are read and written a row at a time, a lane a column.
+//               Sixteen epilogue warps that empty the accumulator at once were no faster (232 against 227 us at
+//               17280 × 8960 × 1536): what bounds the product is the traffic from L2 to the SMs, 64 KB a tile and step.
 // Tensor memory (512 columns): accumulator 0 in [0, 256), accumulator 1 in [240, 496), the scales in [496, 508). The two
 // accumulators share 16 columns, which an epilogue reads first and releases (ovl) before anything else, so the next
 // tile's MMAs start some hundred cycles into the epilogue and run beside the rest of it.
@@ -34,6 +37,7 @@
 #include "../../include/fvsr_lcsa.h"
 #include "common.cuh"
 #include "fp8.cuh"
+#include "fp8_epilogue.cuh"
 #include "sm100.cuh"
 
 namespace fvsr {
@@ -65,24 +69,6 @@ constexpr uint32_t kOffAbort = kOffTmemSlot + 4;
 constexpr uint32_t kOffCols = (kOffAbort + 4 + 15) & ~15u;  // bias[256], gate[256] as fp32
 constexpr uint32_t kSmemBytes = 1024 + kOffCols + 2 * kBN * 4;
 static_assert(kSmemBytes <= 232448, "shared memory");
-
-// GELU with the tanh approximation, 0.5·x·(1 + tanh(√(2/π)·(x + 0.044715·x³))) = x / (1 + 2^z), z = x·(c0 + c1·x²),
-// c0 = −2·√(2/π)·log2(e), c1 = 0.044715·c0; 2^z overflowing gives −0, underflowing gives x.
-__device__ __forceinline__ float gelu_tanh(float x) {
-    constexpr float c0 = -2.0f * 0.7978845608028654f * 1.4426950408889634f, c1 = 0.044715f * c0;
-    return x * rcp_approx(1.0f + ex2_approx(x * fmaf(c1, x * x, c0)));
-}
-
-// What becomes of an accumulator: first / last chain of its sum, add = a value to add (the residual, or what the chains
-// before left).
-template <int kMode>
-__device__ __forceinline__ float finish(float acc, float bias, float gate, float add, bool first, bool last) {
-    float y = first ? acc + bias : acc;
-    if (kMode == FVSR_LINEAR_GATED_RESIDUAL) y *= gate;
-    y += add;
-    if (kMode == FVSR_LINEAR_GELU && last) y = gelu_tanh(y);
-    return y;
-}
 
 struct Work {
     int mt, nt, kt, splits, part_blocks, chain_blocks;
@@ -220,7 +206,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     } else {
         // ---------------- epilogue: this CTA's 128 rows; thread = row = TMEM lane, half = which 128 columns ----------------
         const int quarter = warp & 3, half = (warp - 2) >> 2;
-        const int r = quarter * 32 + lane;
         const int et = threadIdx.x - 64;
         const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * (kBN / 2));
         float* bias_s = reinterpret_cast<float*>(smem + kOffCols);
@@ -248,7 +233,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             for (int cb = kb0; cb < kb1; cb += wk.chain_blocks, ++lt) {
                 const int acc = lt & 1;
                 const bool first = cb == kb0, last = cb + wk.chain_blocks >= kb1;
-                const bool src = !first || kMode == FVSR_LINEAR_GATED_RESIDUAL;  // something to add: chains before, resid
+                // something to add: the chains before (an fp32 output's), the residual
+                const bool src = kMode == FVSR_LINEAR_GATED_RESIDUAL || (!kBf16 && !first);
                 // accumulator 0 from its last chunk to its first, accumulator 1 from its first: the shared columns come first
                 auto chunk = [&](int i) { return acc ? i : kBN / 64 - 1 - i; };
                 auto live = [&](int c) { return row0 < a.M && c0 + 32 * c < a.N; };
@@ -285,61 +271,96 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                         }
                         return;
                     }
-                    if (wk.tma) {
-                        const int place_i = i % kRoom;
-                        uint8_t* mine = chunks + place_i * kChunkBytes + (uint32_t)lane * kRowBytes;
+                    const int place_i = i % kRoom;
+                    uint8_t* const room = chunks + place_i * kChunkBytes;
+                    uint8_t* const mine = room + (uint32_t)lane * kRowBytes;
+                    // without TMA: lane = column, row by row (each element always the same lane's)
+                    const int rows = min(32, a.M - row0);
+                    const bool col_here = c0 + 32 * c + lane < a.N;
+                    const int64_t corner = (int64_t)row0 * a.N + c0 + 32 * c + lane;
+                    auto element = [&](int r) {
+                        const uint32_t byte = (uint32_t)lane * (uint32_t)sizeof(T);
+                        const uint32_t word = (byte >> 4) ^ (kBf16 ? (uint32_t)r >> 1 & 3u : (uint32_t)r & 7u);
+                        return reinterpret_cast<T*>(room + (uint32_t)r * kRowBytes + (word << 4) + (byte & 15u));
+                    };
+                    if (wk.tma && src) {
+                        const bool here = wait(src_bar + place_i, src_phase >> place_i);
+                        src_phase ^= 1u << place_i;
+                        if (!__all_sync(0xffffffffu, here)) ok = false;
+                    } else if (wk.tma) {
+                        if (lane == 0) bulk_wait_read<kRoom - 1>();
+                        __syncwarp();
+                    } else if (src) {
+                        const T* from = (first ? static_cast<const T*>(a.resid) : static_cast<const T*>(a.out)) + corner;
+                        __syncwarp();
+#pragma unroll 1
+                        for (int r0 = 0; r0 < 32; r0 += 16) {
+                            T got[16];  // in flight at once
+#pragma unroll
+                            for (int r = 0; r < 16; ++r)
+                                got[r] = col_here && r0 + r < rows ? from[(int64_t)(r0 + r) * a.N] : T(0.0f);
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) *element(r0 + r) = got[r];
+                        }
+                        __syncwarp();
+                    } else {
+                        __syncwarp();
+                    }
+                    constexpr int kPairs = 8 / sizeof(T);  // of a 16-byte word
+#pragma unroll
+                    for (int w = 0; w < 16 / kPairs; ++w) {
+                        uint4* at = reinterpret_cast<uint4*>(mine + (((uint32_t)w << 4) ^ swizzle));
+                        uint64_t add[kPairs] = {}, y[kPairs];
                         if (src) {
-                            const bool here = wait(src_bar + place_i, src_phase >> place_i);
-                            src_phase ^= 1u << place_i;
-                            if (!__all_sync(0xffffffffu, here)) ok = false;
-                        } else {
-                            if (lane == 0) bulk_wait_read<kRoom - 1>();
-                            __syncwarp();
-                        }
-                        constexpr int kWord = 16 / sizeof(T);
-#pragma unroll
-                        for (int w = 0; w < 32 / kWord; ++w) {
-                            uint4* at = reinterpret_cast<uint4*>(mine + (((uint32_t)w << 4) ^ swizzle));
-                            float add[kWord] = {}, y[kWord];
-                            if (src) {
+                            if constexpr (kBf16) {
                                 const uint4 u = *at;
-                                if constexpr (kBf16) {
-                                    bf2_to_f(u.x, add[0], add[1]), bf2_to_f(u.y, add[2], add[3]);
-                                    bf2_to_f(u.z, add[4], add[5]), bf2_to_f(u.w, add[6], add[7]);
-                                } else {
-                                    add[0] = __uint_as_float(u.x), add[1] = __uint_as_float(u.y);
-                                    add[2] = __uint_as_float(u.z), add[3] = __uint_as_float(u.w);
-                                }
-                            }
+                                const uint32_t p[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-                            for (int e = 0; e < kWord; ++e)
-                                y[e] = finish<kMode>(__uint_as_float(v[w * kWord + e]), bias[w * kWord + e],
-                                                     gate[w * kWord + e], add[e], kBf16 || first, kBf16 || last);
-                            if constexpr (kBf16)
-                                *at = make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]),
-                                                 pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7]));
-                            else
-                                *at = make_uint4(__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]),
-                                                 __float_as_uint(y[3]));
+                                for (int e = 0; e < kPairs; ++e) {
+                                    float lo, hi;
+                                    bf2_to_f(p[e & 3], lo, hi);
+                                    add[e] = f2(lo, hi);
+                                }
+                            } else {
+                                const ulonglong2 u = *reinterpret_cast<const ulonglong2*>(at);
+                                add[0] = u.x, add[kPairs - 1] = u.y;
+                            }
                         }
+#pragma unroll
+                        for (int e = 0; e < kPairs; ++e) {
+                            const int i = 2 * (w * kPairs + e);
+                            y[e] = finish2<kMode>(f2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])),
+                                                  *reinterpret_cast<const uint64_t*>(bias + i),
+                                                  *reinterpret_cast<const uint64_t*>(gate + i), add[e],
+                                                  kBf16 || first, kBf16 || last);
+                        }
+                        if constexpr (kBf16) {
+                            uint32_t p[4];
+#pragma unroll
+                            for (int e = 0; e < kPairs; ++e) {
+                                float lo, hi;
+                                uf2(y[e], lo, hi);
+                                p[e & 3] = pack_bf16x2(lo, hi);
+                            }
+                            *at = make_uint4(p[0], p[1], p[2], p[3]);
+                        } else {
+                            *reinterpret_cast<ulonglong2*>(at) = make_ulonglong2(y[0], y[kPairs - 1]);
+                        }
+                    }
+                    if (wk.tma) {
                         fence_async_shared();
                         __syncwarp();
                         if (lane == 0) {
-                            tma_store_3d(&tmOut, c0 + 32 * c, row0, plane, smem_u32(mine));
+                            tma_store_3d(&tmOut, c0 + 32 * c, row0, plane, smem_u32(room));
                             bulk_commit();
                             fetch_next();
                         }
-                    } else if (row0 + lane < a.M) {
-                        const int64_t at = (int64_t)(row0 + lane) * a.N + c0 + 32 * c;
-                        T* out = static_cast<T*>(a.out) + at;
-                        const T* from = first ? static_cast<const T*>(a.resid) + at : out;
-                        const int left = a.N - (c0 + 32 * c);
-#pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if (e < left)
-                                store_from_float(out + e, finish<kMode>(__uint_as_float(v[e]), bias[e], gate[e],
-                                                                        src ? load_as_float(from + e) : 0.0f,
-                                                                        kBf16 || first, kBf16 || last));
+                    } else {
+                        __syncwarp();
+                        T* to = static_cast<T*>(a.out) + corner;
+                        if (col_here)
+#pragma unroll 8
+                            for (int r = 0; r < rows; ++r) to[(int64_t)r * a.N] = *element(r);
                     }
                 };
                 uint32_t va[32], vb[32];
@@ -393,16 +414,20 @@ __global__ void __launch_bounds__(256) gemm_fp8_join_kernel(const Fp8GemmArgs a,
         const float4 v = *reinterpret_cast<const float4*>(p + k * plane);
         s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
     }
-    const float v[4] = {s.x, s.y, s.z, s.w};
     T* out = static_cast<T*>(a.out) + row * a.N + col;
     const T* resid = static_cast<const T*>(a.resid) + row * a.N + col;
+    float b[4] = {}, g[4] = {}, r[4] = {}, y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (e >= left) break;
+        if (a.bias) b[e] = __bfloat162float(a.bias[col + e]);
+        if (kMode == FVSR_LINEAR_GATED_RESIDUAL) g[e] = __bfloat162float(a.gate[col + e]), r[e] = load_as_float(resid + e);
+    }
+    uf2(finish2<kMode>(f2(s.x, s.y), f2(b[0], b[1]), f2(g[0], g[1]), f2(r[0], r[1]), true, true), y[0], y[1]);
+    uf2(finish2<kMode>(f2(s.z, s.w), f2(b[2], b[3]), f2(g[2], g[3]), f2(r[2], r[3]), true, true), y[2], y[3]);
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-        if (e < left)
-            store_from_float(out + e,
-                             finish<kMode>(v[e], a.bias ? __bfloat162float(a.bias[col + e]) : 0.0f,
-                                           kMode == FVSR_LINEAR_GATED_RESIDUAL ? __bfloat162float(a.gate[col + e]) : 0.0f,
-                                           kMode == FVSR_LINEAR_GATED_RESIDUAL ? load_as_float(resid + e) : 0.0f, true, true));
+        if (e < left) store_from_float(out + e, y[e]);
 }
 
 struct Maps {
@@ -411,8 +436,8 @@ struct Maps {
 
 template <typename T, int kMode>
 cudaError_t launch_tiles(const Fp8GemmArgs& args, const Work& wk, const Maps& m, cudaStream_t st) {
-    auto kernel = gemm_fp8_sm100_kernel<T, kMode>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes);
+    constexpr auto kernel = gemm_fp8_sm100_kernel<T, kMode>;
+    cudaError_t e = allow_smem<kernel>(kSmemBytes);
     if (e != cudaSuccess) return e;
     const int items = wk.mt * wk.nt * wk.splits, pairs = sm_count() / 2;
     return launch_pdl(kernel, dim3(2 * (items < pairs ? items : pairs)), dim3(kThreads), kSmemBytes, st, m.x, m.w, m.xs,
@@ -447,8 +472,11 @@ Fp8GemmPlan plan_gemm_fp8(int M, int N, int K) {
     const int kt = (K + kBK - 1) / kBK, groups = (kt + 3) / 4;
     const int64_t tiles = (int64_t)((M + kBM - 1) / kBM) * ((N + kBN - 1) / kBN);
     const int pairs = sm_count() / 2;
+    // Parts of at least 1024 along K: with 512 the join costs more than it gives (777 × 1000 × 1100 12.3 against 10.8 us,
+    // 17 × 9216 × 1536 11.5 / 10.0, but 17 × 1536 × 1536 9.2 / 9.8); with 1536 the parts get too few (17 × 1536 × 8960
+    // 11.1 against 12.5 us, 300 × 300 × 4000 12.6 / 14.9).
     int splits = tiles * 2 <= pairs ? (int)(pairs / tiles) : 1;
-    if (splits > groups) splits = groups;
+    if (splits > groups / 2) splits = groups < 2 ? 1 : groups / 2;
     const int per = (groups + splits - 1) / splits;
     p.splits = (groups + per - 1) / per;
     p.part_blocks = 4 * per;

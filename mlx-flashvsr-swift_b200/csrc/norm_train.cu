@@ -458,10 +458,10 @@ struct Shape {
         return (int)(need < most ? need : most);
     }
 };
-template <typename Kernel>
-cudaError_t launch_ring(Kernel kernel, int ctas, const Shape& s, size_t ring_bytes, const NormTrainArgs& a, cudaStream_t st) {
+template <auto kernel>
+cudaError_t launch_ring(int ctas, const Shape& s, size_t ring_bytes, const NormTrainArgs& a, cudaStream_t st) {
     if (ring_bytes > 40 * 1024) {
-        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ring_bytes);
+        cudaError_t e = allow_smem<kernel>(ring_bytes);
         if (e != cudaSuccess) return e;
     }
     return launch_pdl(kernel, dim3(ctas), dim3(s.threads), ring_bytes, st, a, s.tpr);
@@ -473,20 +473,20 @@ cudaError_t train(const NormTrainArgs& a, cudaStream_t st) {
     const Shape s(a.c);
     const int rows = a.c > kWideC ? 1 : kRows, ctas = s.ctas(a.m, rows, kForwardThreads);
     const size_t ring = (size_t)kStages * rows * s.most_threads() * 8 * sizeof(T);
-    if (s.threads <= 192) return launch_ring(norm_train_kernel<T, kVec, kRows, 192>, ctas, s, ring, a, st);
-    if (s.threads <= 256) return launch_ring(norm_train_kernel<T, kVec, kRows, 256>, ctas, s, ring, a, st);
-    if (a.c <= kWideC) return launch_ring(norm_train_kernel<T, kVec, kRows, 512>, ctas, s, ring, a, st);
-    return launch_ring(norm_train_kernel<T, kVec, 1, 1024>, ctas, s, ring, a, st);
+    if (s.threads <= 192) return launch_ring<norm_train_kernel<T, kVec, kRows, 192>>(ctas, s, ring, a, st);
+    if (s.threads <= 256) return launch_ring<norm_train_kernel<T, kVec, kRows, 256>>(ctas, s, ring, a, st);
+    if (a.c <= kWideC) return launch_ring<norm_train_kernel<T, kVec, kRows, 512>>(ctas, s, ring, a, st);
+    return launch_ring<norm_train_kernel<T, kVec, 1, 1024>>(ctas, s, ring, a, st);
 }
 
 template <typename T, bool kHeld, bool kVec>
 cudaError_t backward_rows(const NormTrainArgs& a, const Shape& s, int ctas, cudaStream_t st) {
     constexpr int kRows = kBackwardRows;
     const size_t ring = (size_t)kStages * (a.c > kWideC ? 1 : kRows) * s.most_threads() * 8 * (sizeof(T) + (kHeld ? 1 : sizeof(T)));
-    if (s.threads <= 192) return launch_ring(norm_backward_kernel<T, kHeld, kVec, kRows, 192>, ctas, s, ring, a, st);
-    if (s.threads <= 256) return launch_ring(norm_backward_kernel<T, kHeld, kVec, kRows, 256>, ctas, s, ring, a, st);
-    if (a.c <= kWideC) return launch_ring(norm_backward_kernel<T, kHeld, kVec, kRows, 512>, ctas, s, ring, a, st);
-    return launch_ring(norm_backward_kernel<T, kHeld, kVec, 1, 1024>, ctas, s, ring, a, st);
+    if (s.threads <= 192) return launch_ring<norm_backward_kernel<T, kHeld, kVec, kRows, 192>>(ctas, s, ring, a, st);
+    if (s.threads <= 256) return launch_ring<norm_backward_kernel<T, kHeld, kVec, kRows, 256>>(ctas, s, ring, a, st);
+    if (a.c <= kWideC) return launch_ring<norm_backward_kernel<T, kHeld, kVec, kRows, 512>>(ctas, s, ring, a, st);
+    return launch_ring<norm_backward_kernel<T, kHeld, kVec, 1, 1024>>(ctas, s, ring, a, st);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }

@@ -331,10 +331,10 @@ __global__ void __launch_bounds__(kThreads) codes_kernel(int64_t rows, int64_t b
 template <typename T, bool kVec, bool kTrans>
 cudaError_t quantize(int64_t rows, int64_t cols, const T* x, bool square, uint8_t* q, uint8_t* scale, uint8_t* qt,
                      uint8_t* scale_t, cudaStream_t st) {
-    auto kernel = quantize_kernel<T, kVec, kTrans>;
+    constexpr auto kernel = quantize_kernel<T, kVec, kTrans>;
     const size_t smem = kTrans ? sizeof(T) * kT * kT : 0;
     if (smem > 48 * 1024) {
-        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        cudaError_t e = allow_smem<kernel>(smem);
         if (e != cudaSuccess) return e;
     }
     const int64_t tiles = (rows + kT - 1) / kT * ((cols + kT - 1) / kT);

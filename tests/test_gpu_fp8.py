@@ -129,7 +129,7 @@ def _held_to(got, want, size, k, epilogue, gate, dtype):
 LINEARS = [(1, 1, 1), (1, 16, 128), (1, 1536, 1536), (1, 77, 1100), (2, 300, 257), (5, 1000, 640), (8, 9216, 1536),
            (16, 129, 4100), (17, 256, 128), (31, 500, 700), (64, 64, 512), (127, 255, 384), (128, 256, 128),
            (129, 257, 129), (200, 1, 1000), (256, 512, 1536), (300, 8, 64), (777, 1000, 1100), (1025, 768, 2500),
-           (2048, 1536, 1536), (300, 200, 9000), (1536, 1536, 5000), (2600, 1100, 4700), (2600, 1102, 8300), (4000, 1604, 300)]
+           (2048, 1536, 1536), (300, 200, 9000), (1536, 1536, 5000), (2600, 1100, 4700), (2600, 1102, 8300), (4000, 1604, 300), (300, 301, 4000)]
 
 
 @pytest.mark.parametrize("m,n,k", LINEARS)
