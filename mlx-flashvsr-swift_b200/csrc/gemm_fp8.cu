@@ -9,9 +9,8 @@
 // registers, and a weight gradient (a scale for each row and block on both sides) costs what a forward product does.
 //
 // Persistent kernel over CTA pairs (clusters of two CTAs, one TPC): a pair walks 256 × 256 output tiles, CTA r of it
-// loading rows [m0 + 128r, +128) of x and [n0 + 128r, +128) of w per 128-wide K step (32 KB a stage, 4 stages: measured
-// no slower than 5 or 6) and, every fourth step, the codes of its 128 rows of x and of all 256 rows of w. Warp roles (320
-// threads per CTA):
+// loading rows [m0 + 128r, +128) of x and [n0 + 128r, +128) of w per 128-wide K step (32 KB a stage, 5 stages) and, every
+// fourth step, the codes of its 128 rows of x and of all 256 rows of w. Warp roles (320 threads per CTA):
 //   warp 0      TMA producer;
 //   warp 1      TMEM owner and, in the even CTA, the issuer of the scale copies and MMAs (M 256, N 256, K 32);
 //   warps 2..9  epilogue: thread = output row = TMEM lane, each half of the warps 128 of the tile's columns, 32 at a time
@@ -20,11 +19,15 @@
 //               is written to. (Stores straight from the threads, a row each and 32 rows an instruction, cost 13 % of
 //               the whole product at K = 1536.) Rows that are not 16-byte aligned take the same way through shared
 //               memory and are read and written a row at a time, a lane a column.
-//               Sixteen epilogue warps that empty the accumulator at once were no faster (232 against 227 us at
-//               17280 × 8960 × 1536): what bounds the product is the traffic from L2 to the SMs, 64 KB a tile and step.
+// The first two warps walk the tiles as whole warps and issue under elect_one: issued by `lane == 0`, a step's four MMAs
+// and its wait took 720 cycles instead of the MMAs' 512, whatever the ring's depth.
 // Tensor memory (512 columns): accumulator 0 in [0, 256), accumulator 1 in [240, 496), the scales in [496, 508). The two
 // accumulators share 16 columns, which an epilogue reads first and releases (ovl) before anything else, so the next
 // tile's MMAs start some hundred cycles into the epilogue and run beside the rest of it.
+// Measured at 17280 × 8960 × 1536 from 8-bit operands, and what was not kept: 4 stages 171 us, 5 164, 6 (no room for two
+// chunks a warp) 160, GELU 200, 203 and 208 (all at the full clock, on zeros; at the power limit, on random values, 197,
+// 195, 193 and 237, 232, 241); tiles of 256 × 384 in two accumulators of 192 columns 183; sixteen epilogue warps 191
+// (GELU 183). On random values the clock falls to 1.5 GHz at 1000 W, so energy a product decides there.
 //
 // The tensor core adds to its fp32 accumulator by truncation, an error that grows with the number of additions (measured
 // relative to the result: 2e-7 after K = 4096, 1.3e-6 after 17280, on zero-mean operands; a bf16 output does not see it).
@@ -48,7 +51,7 @@ namespace {
 
 using namespace sm100;
 
-constexpr int kBM = 256, kBN = 256, kBK = 128, kStages = 4;
+constexpr int kBM = 256, kBN = 256, kBK = 128, kStages = 5;
 constexpr uint32_t kHalfBytes = 128 * kBK;       // 16 KB: one CTA's rows of x or of w per K step
 constexpr uint32_t kStageBytes = 2 * kHalfBytes;
 constexpr uint32_t kScaleBytes = 3 * 512;        // x's 128 rows, w's 256 rows, four blocks
@@ -58,9 +61,9 @@ constexpr int kChainBlocks = 32;                 // of 128: the longest chain of
 constexpr uint64_t kWaitLimitNs = 4000000000ull;
 constexpr uint32_t kIdesc = idesc_mxf8(kBM, kBN);
 constexpr uint32_t kAcc1 = 240, kTmemScale = 496;
-constexpr uint32_t kChunkRoom = 8192;            // an epilogue warp's chunks: 4 of 32 × 32 bf16 or 2 of fp32
+constexpr uint32_t kChunkRoom = 4096;            // an epilogue warp's chunks: 2 of 32 × 32 bf16 or 1 of fp32
 constexpr int kBarFull = 0, kBarEmpty = kStages, kBarAccFull = 2 * kStages, kBarAccEmpty = 2 * kStages + 2,
-              kBarOvl = 2 * kStages + 4, kBarSrc = 2 * kStages + 5, kNumBars = kBarSrc + 4 * kEpiWarps;
+              kBarOvl = 2 * kStages + 4, kBarSrc = 2 * kStages + 5, kNumBars = kBarSrc + 2 * kEpiWarps;
 constexpr uint32_t kOffChunks = kStages * kStageBytes;
 constexpr uint32_t kOffScale = kOffChunks + kEpiWarps * kChunkRoom;
 constexpr uint32_t kOffBar = kOffScale + kStages * kScaleBytes;
@@ -94,6 +97,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     auto wait = [&](int b, uint32_t parity) {
         return mbar_wait(bar(b), parity & 1u, abort_word, &g_gemm_fp8_timeout, kWaitLimitNs);
     };
+    // for a whole warp
+    auto wait_all = [&](int b, uint32_t parity) { return __all_sync(0xffffffffu, wait(b, parity)) != 0; };
     // item → output tile (columns fastest) and blocks [kb0, kb1) of K
     auto place = [&](int t, int& m0, int& n0, int& kb0, int& kb1) {
         const int tile = t / wk.splits, part = t % wk.splits;
@@ -110,7 +115,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             mbar_init(bar(kBarAccEmpty + b), 2 * kEpiWarps);
         }
         mbar_init(bar(kBarOvl), kEpiWarps);
-        for (int b = 0; b < 4 * kEpiWarps; ++b) mbar_init(bar(kBarSrc + b), 1);
+        for (int b = 0; b < 2 * kEpiWarps; ++b) mbar_init(bar(kBarSrc + b), 1);
         *abort_word = 0;
         fence_mbar_init();
     }
@@ -133,7 +138,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
     if (warp == 0) {
         // ---------------- TMA producer: rows past the tensors' ends read as zeros with scale code 0 ----------------
-        if (lane == 0) {
+        {
+            const bool issuer = elect_one();
             uint32_t it = 0;
             bool ok = true;
             for (int t = pair; ok && t < items; t += npairs) {
@@ -143,11 +149,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 const int nr = n0 + 128 * (int)rank;
                 for (int kb = kb0; kb < kb1; ++kb, ++it) {
                     const int st = (int)(it % kStages);
-                    if (it >= kStages && !(ok = wait(kBarEmpty + st, it / kStages - 1))) break;
+                    if (it >= kStages && !(ok = wait_all(kBarEmpty + st, it / kStages - 1))) break;
                     const uint32_t dst = sbase + (uint32_t)st * kStageBytes;
                     const uint32_t sdst = sbase + kOffScale + (uint32_t)st * kScaleBytes;
                     const uint32_t full0 = mapa_shared(bar(kBarFull + st), 0);
                     const bool scales = (kb & 3) == 0;
+                    if (!issuer) continue;
                     if (rank == 0) mbar_expect_tx(bar(kBarFull + st), 2 * (kStageBytes + (scales ? kScaleBytes : 0)));
                     tma_load_2d_pair(dst, &tmX, kb * kBK, m0, full0);
                     tma_load_2d_pair(dst + kHalfBytes, &tmW, kb * kBK, nr, full0);
@@ -161,8 +168,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             }
         }
     } else if (warp == 1) {
-        // ---------------- MMA issuer: one thread of the even CTA ----------------
-        if (lane == 0 && rank == 0) {
+        // ---------------- MMA issuer: one lane of the even CTA, its warp walking the tiles with it ----------------
+        if (rank == 0) {
+            const bool issuer = elect_one();
             uint32_t it = 0;
             bool ok = true;
             int lt = 0;
@@ -171,14 +179,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 place(t, m0, n0, kb0, kb1);
                 for (int cb = kb0; ok && cb < kb1; cb += wk.chain_blocks, ++lt) {
                     const int acc = lt & 1, ce = min(cb + wk.chain_blocks, kb1);
-                    if (lt >= 2 && !(ok = wait(kBarAccEmpty + acc, (uint32_t)((lt >> 1) - 1)))) break;
-                    if (lt >= 1 && !(ok = wait(kBarOvl, (uint32_t)(lt - 1)))) break;
+                    if (lt >= 2 && !(ok = wait_all(kBarAccEmpty + acc, (uint32_t)((lt >> 1) - 1)))) break;
+                    if (lt >= 1 && !(ok = wait_all(kBarOvl, (uint32_t)(lt - 1)))) break;
                     tc_fence_after();
                     const uint32_t d = tmem + (acc ? kAcc1 : 0u), sf = tmem + kTmemScale;
                     for (int kb = cb; kb < ce; ++kb, ++it) {
                         const int st = (int)(it % kStages);
-                        if (!(ok = wait(kBarFull + st, it / kStages))) break;
+                        if (!(ok = wait_all(kBarFull + st, it / kStages))) break;
                         tc_fence_after();
+                        if (!issuer) continue;
                         const uint32_t sa = sbase + (uint32_t)st * kStageBytes;
                         if ((kb & 3) == 0) {
                             const uint32_t sc = sbase + kOffScale + (uint32_t)st * kScaleBytes;
@@ -193,13 +202,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                         for (int kk = 0; kk < kBK / 32; ++kk)
                             mma_mxf8_pair(d, ad + (uint64_t)(2 * kk), bd + (uint64_t)(2 * kk), idesc, sf, sf + 4,
                                           (kb > cb || kk > 0) ? 1u : 0u);
-                        mma_commit_pair(bar(kBarEmpty + st));
-                        mma_commit_pair(mapa_shared(bar(kBarEmpty + st), 1));
+                        mma_commit_both(bar(kBarEmpty + st));
                     }
-                    if (ok) {
-                        mma_commit_pair(bar(kBarAccFull + acc));
-                        mma_commit_pair(mapa_shared(bar(kBarAccFull + acc), 1));
-                    }
+                    if (ok && issuer) mma_commit_both(bar(kBarAccFull + acc));
                 }
             }
         }
@@ -212,11 +217,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         float* gate_s = bias_s + kBN;
         const uint32_t acc_empty0 = mapa_shared(bar(kBarAccEmpty), 0), ovl0 = mapa_shared(bar(kBarOvl), 0);
         constexpr bool kBf16 = sizeof(T) == 2;
-        constexpr int kRoom = kBf16 ? 4 : 2;  // chunks in flight
+        constexpr bool kAdds = !kBf16 || kMode == FVSR_LINEAR_GATED_RESIDUAL;  // something may be added to the products
+        constexpr int kRoom = kBf16 ? 2 : 1;  // chunks in flight
         constexpr uint32_t kRowBytes = 32 * sizeof(T), kChunkBytes = 32 * kRowBytes;
         uint8_t* const chunks = smem + kOffChunks + (uint32_t)(warp - 2) * kChunkRoom;
         const uint32_t swizzle = (kBf16 ? (uint32_t)lane >> 1 & 3u : (uint32_t)lane & 7u) << 4;
-        const int src_bar = kBarSrc + 4 * (warp - 2);
+        const int src_bar = kBarSrc + 2 * (warp - 2);
         uint32_t src_phase = 0;  // bit b: parity of the next wait on chunk place b
         int lt = 0;
         bool ok = true;
@@ -234,7 +240,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 const int acc = lt & 1;
                 const bool first = cb == kb0, last = cb + wk.chain_blocks >= kb1;
                 // something to add: the chains before (an fp32 output's), the residual
-                const bool src = kMode == FVSR_LINEAR_GATED_RESIDUAL || (!kBf16 && !first);
+                const bool src = kAdds && (kMode == FVSR_LINEAR_GATED_RESIDUAL || !first);
                 // accumulator 0 from its last chunk to its first, accumulator 1 from its first: the shared columns come first
                 auto chunk = [&](int i) { return acc ? i : kBN / 64 - 1 - i; };
                 auto live = [&](int c) { return row0 < a.M && c0 + 32 * c < a.N; };
@@ -329,7 +335,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
                         for (int e = 0; e < kPairs; ++e) {
                             const int i = 2 * (w * kPairs + e);
-                            y[e] = finish2<kMode>(f2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])),
+                            y[e] = finish2<kMode, kAdds>(f2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])),
                                                   *reinterpret_cast<const uint64_t*>(bias + i),
                                                   *reinterpret_cast<const uint64_t*>(gate + i), add[e],
                                                   kBf16 || first, kBf16 || last);
@@ -423,8 +429,8 @@ __global__ void __launch_bounds__(256) gemm_fp8_join_kernel(const Fp8GemmArgs a,
         if (a.bias) b[e] = __bfloat162float(a.bias[col + e]);
         if (kMode == FVSR_LINEAR_GATED_RESIDUAL) g[e] = __bfloat162float(a.gate[col + e]), r[e] = load_as_float(resid + e);
     }
-    uf2(finish2<kMode>(f2(s.x, s.y), f2(b[0], b[1]), f2(g[0], g[1]), f2(r[0], r[1]), true, true), y[0], y[1]);
-    uf2(finish2<kMode>(f2(s.z, s.w), f2(b[2], b[3]), f2(g[2], g[3]), f2(r[2], r[3]), true, true), y[2], y[3]);
+    uf2(finish2<kMode, kMode == FVSR_LINEAR_GATED_RESIDUAL>(f2(s.x, s.y), f2(b[0], b[1]), f2(g[0], g[1]), f2(r[0], r[1]), true, true), y[0], y[1]);
+    uf2(finish2<kMode, kMode == FVSR_LINEAR_GATED_RESIDUAL>(f2(s.z, s.w), f2(b[2], b[3]), f2(g[2], g[3]), f2(r[2], r[3]), true, true), y[2], y[3]);
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         if (e < left) store_from_float(out + e, y[e]);

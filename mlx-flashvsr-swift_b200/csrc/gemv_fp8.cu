@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(512) gemv_fp8_kernel(const Fp8GemmArgs a, cons
         float gate = 0.0f, add = 0.0f, y, unused;
         if (kMode == FVSR_LINEAR_GATED_RESIDUAL)
             gate = __bfloat162float(a.gate[n]), add = load_as_float(static_cast<const T*>(a.resid) + at);
-        uf2(finish2<kMode>(f2(s, s), f2(bias, bias), f2(gate, gate), f2(add, add), true, true), y, unused);
+        uf2(finish2<kMode, kMode == FVSR_LINEAR_GATED_RESIDUAL>(f2(s, s), f2(bias, bias), f2(gate, gate), f2(add, add), true, true), y, unused);
         store_from_float(static_cast<T*>(a.out) + at, y);
     }
 }
