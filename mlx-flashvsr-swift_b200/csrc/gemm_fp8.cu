@@ -216,6 +216,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         float* bias_s = reinterpret_cast<float*>(smem + kOffCols);
         float* gate_s = bias_s + kBN;
         const uint32_t acc_empty0 = mapa_shared(bar(kBarAccEmpty), 0), ovl0 = mapa_shared(bar(kBarOvl), 0);
+        const bool leader = elect_one();  // issues the warp's copies and signals
         constexpr bool kBf16 = sizeof(T) == 2;
         constexpr bool kAdds = !kBf16 || kMode == FVSR_LINEAR_GATED_RESIDUAL;  // something may be added to the products
         constexpr int kRoom = kBf16 ? 2 : 1;  // chunks in flight
@@ -244,7 +245,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 // accumulator 0 from its last chunk to its first, accumulator 1 from its first: the shared columns come first
                 auto chunk = [&](int i) { return acc ? i : kBN / 64 - 1 - i; };
                 auto live = [&](int c) { return row0 < a.M && c0 + 32 * c < a.N; };
-                auto fetch = [&](int i) {  // by lane 0: the values to add to chunk i into its place
+                auto fetch = [&](int i) {  // by the leader: the values to add to chunk i into its place
                     const int c = chunk(i);
                     if (!live(c)) return;
                     const uint32_t b = bar(src_bar + i % kRoom);
@@ -252,7 +253,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     tma_load_3d(smem_u32(chunks + (i % kRoom) * kChunkBytes), first ? &tmResid : &tmOut, c0 + 32 * c,
                                 row0, plane, b);
                 };
-                if (wk.tma && src && ok && lane == 0) {
+                if (wk.tma && src && ok && leader) {
                     if (first) bulk_wait_read<0>();
                     else bulk_wait<0>();  // the chain before is in memory
                     for (int i = 0; i < kRoom; ++i) fetch(i);
@@ -264,14 +265,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 auto emit = [&](const uint32_t* v, int i) {
                     const int c = chunk(i);
                     const float *bias = bcol + 32 * c, *gate = gcol + 32 * c;
-                    auto fetch_next = [&] {  // by lane 0, once this chunk's place is free again
+                    auto fetch_next = [&] {  // by the leader, once this chunk's place is free again
                         if (src && i + kRoom < kBN / 64) {
                             bulk_wait_read<0>();
                             fetch(i + kRoom);
                         }
                     };
                     if (!live(c)) {
-                        if (wk.tma && lane == 0) {
+                        if (wk.tma && leader) {
                             bulk_commit();  // keeps the groups' count
                             fetch_next();
                         }
@@ -294,7 +295,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                         src_phase ^= 1u << place_i;
                         if (!__all_sync(0xffffffffu, here)) ok = false;
                     } else if (wk.tma) {
-                        if (lane == 0) bulk_wait_read<kRoom - 1>();
+                        if (leader) bulk_wait_read<kRoom - 1>();
                         __syncwarp();
                     } else if (src) {
                         const T* from = (first ? static_cast<const T*>(a.resid) : static_cast<const T*>(a.out)) + corner;
@@ -356,7 +357,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     if (wk.tma) {
                         fence_async_shared();
                         __syncwarp();
-                        if (lane == 0) {
+                        if (leader) {
                             tma_store_3d(&tmOut, c0 + 32 * c, row0, plane, smem_u32(room));
                             bulk_commit();
                             fetch_next();
@@ -375,7 +376,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 if (half != acc) {  // this half held the shared columns: half 1 of accumulator 0, half 0 of accumulator 1
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive_cluster(ovl0);
+                    if (leader) mbar_arrive_cluster(ovl0);
                 }
 #pragma unroll
                 for (int i = 0; i < kBN / 64; i += 2) {
@@ -386,14 +387,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     if (i + 2 == kBN / 64) {  // the accumulator is in registers
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive_cluster(acc_empty0 + 8u * (uint32_t)acc);
+                        if (leader) mbar_arrive_cluster(acc_empty0 + 8u * (uint32_t)acc);
                     }
                     emit(vb, i + 1);
                     if (i + 2 < kBN / 64) tmem_ld_wait(va);
                 }
             }
         }
-        if (wk.tma && lane == 0) bulk_wait<0>();
+        if (wk.tma && leader) bulk_wait<0>();
     }
     tc_fence_before();
     cluster_sync();  // no signal to the other CTA and no MMA on this CTA's shared memory is still in flight
