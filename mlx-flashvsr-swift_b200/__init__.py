@@ -948,7 +948,8 @@ def layernorm_train(x, weight=None, bias=None, shift=None, scale=None, eps: floa
     weight, bias = _channel_vector(weight, "weight", c, dt, x), _channel_vector(bias, "bias", c, dt, x)
     shift, scale = _channel_vector(shift, "shift", c, dt, x), _channel_vector(scale, "scale", c, dt, x)
     out = _torch().empty_like(x) if out is None else _matrix(out, "out", dtypes=(dt,), shape=x.shape, like=x)
-    mean, rstd = x.new_empty((m,), dtype=f32), x.new_empty((m,), dtype=f32)
+    mean = x.new_empty((m,), dtype=f32)
+    rstd = _torch().empty_like(mean)
     _check(lib().fvsr_layernorm_train(m, c, x.data_ptr(), _dtype_code(x), weight, bias, shift, scale, eps,
                                       out.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _here(x)))
     return out, mean, rstd
@@ -974,8 +975,11 @@ def layernorm_backward(dy, x, mean, rstd, weight=None, bias=None, scale=None, dx
     if mean is None or rstd is None:
         raise FVSRError(FVSR_EINVAL, "mean and rstd are required")
     grads = {"dx": _torch().empty_like(dy) if dx is None else _matrix(dx, "dx", dtypes=(dt,), shape=dy.shape, like=dy)}
+    like = None
     for name, given in (("dweight", weight), ("dbias", weight), ("dscale", scale), ("dshift", scale)):
-        grads[name] = None if given is None else dy.new_empty((c,), dtype=f32)
+        grads[name] = None
+        if given is not None:
+            grads[name] = like = dy.new_empty((c,), dtype=f32) if like is None else _torch().empty_like(like)
     weight, bias = _channel_vector(weight, "weight", c, dt, dy), _channel_vector(bias, "bias", c, dt, dy)
     scale = _channel_vector(scale, "scale", c, dt, dy)
     need = _bytes("fvsr_layernorm_backward_workspace_size", dy.get_device(), m, c) if workspace is None else 0

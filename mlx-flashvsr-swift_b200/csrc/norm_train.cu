@@ -24,11 +24,14 @@ namespace {
 
 using namespace sm100;
 
-__device__ __forceinline__ void copy_async16(void* dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+// Asynchronous copies of 16 or 8 bytes, or as many zeros without a source (here false: src is not read).
+__device__ __forceinline__ void copy_async16(void* dst, const void* src, bool here) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(here ? 16 : 0)
+                 : "memory");
 }
-__device__ __forceinline__ void copy_async8(void* dst, const void* src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+__device__ __forceinline__ void copy_async8(void* dst, const void* src, bool here) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(here ? 8 : 0)
+                 : "memory");
 }
 __device__ __forceinline__ void copy_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int kPending>
@@ -49,10 +52,8 @@ template <typename T, bool kVec>
 __device__ __forceinline__ void fetch8(const T* p, int n, uint4* w, int stride) {
     if constexpr (kVec) {
 #pragma unroll
-        for (int i = 0; i < Piece<T>::kWords; ++i) {
-            if (n > 0) copy_async16(w + i * stride, reinterpret_cast<const uint4*>(p) + i);
-            else w[i * stride] = make_uint4(0, 0, 0, 0);
-        }
+        for (int i = 0; i < Piece<T>::kWords; ++i)
+            copy_async16(w + i * stride, reinterpret_cast<const uint4*>(p) + i, n > 0);
     } else {
         alignas(16) T v[8];
 #pragma unroll
@@ -280,8 +281,7 @@ __global__ void __launch_bounds__(kMaxThreads, kBackwardThreads / kMaxThreads > 
             fetch8<T, kVec>(dy + fetch_at + i * c, here, mine + (stage * kRows + i) * kRowWords, kMaxThreads);
             if constexpr (kHeld) {
                 uint2* to = mine_x8 + (stage * kRows + i) * kMaxThreads;
-                if (here > 0) copy_async8(to, x8 + fetch_at8 + i * ld);
-                else *to = make_uint2(0, 0);
+                copy_async8(to, x8 + fetch_at8 + i * ld, here > 0);
             } else {
                 fetch8<T, kVec>(x + fetch_at + i * c, here, mine_x + (stage * kRows + i) * kRowWords, kMaxThreads);
             }
@@ -290,19 +290,17 @@ __global__ void __launch_bounds__(kMaxThreads, kBackwardThreads / kMaxThreads > 
         fetch_at += step * c;
         if (kHeld) fetch_at8 += step * ld;
     };
-    // the rows' statistics (and codes) one step ahead, in registers
+    // the rows' statistics (and codes) one step ahead, in registers; past the last row, that row's: its dy there is zero
     float next_mean[kRows], next_rstd[kRows];
     uint32_t next_code[kRows];
+    const int tile_bytes = (int)fp8_scale_tiles(a.c) * 512, block = min(col, a.c - 1) >> 7;
+    const uint8_t* codes = kHeld ? a.x_scale + (block >> 2) * 512 + (block & 3) : nullptr;
     auto fetch_row = [&](int rows) {
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
-            next_mean[i] = next_rstd[i] = 0.0f;
-            next_code[i] = 0;
-            if (i < rows) {
-                const int r = m - rows + i;
-                next_mean[i] = a.mean[r], next_rstd[i] = a.rstd[r];
-                if (kHeld && n > 0) next_code[i] = a.x_scale[fp8_code_pos(r, col >> 7, fp8_scale_tiles(a.c))];
-            }
+            const int r = min(m - rows + i, m - 1);
+            next_mean[i] = a.mean[r], next_rstd[i] = a.rstd[r];
+            if (kHeld) next_code[i] = codes[(int64_t)(r >> 7) * tile_bytes + (r & 31) * 16 + ((r >> 5) & 3) * 4];
         }
     };
     griddep_wait_then_release();
