@@ -24,10 +24,13 @@
 // Tensor memory (512 columns): accumulator 0 in [0, 256), accumulator 1 in [240, 496), the scales in [496, 508). The two
 // accumulators share 16 columns, which an epilogue reads first and releases (ovl) before anything else, so the next
 // tile's MMAs start some hundred cycles into the epilogue and run beside the rest of it.
-// Measured at 17280 × 8960 × 1536 from 8-bit operands, and what was not kept: 4 stages 171 us, 5 164, 6 (no room for two
-// chunks a warp) 160, GELU 200, 203 and 208 (all at the full clock, on zeros; at the power limit, on random values, 197,
-// 195, 193 and 237, 232, 241); tiles of 256 × 384 in two accumulators of 192 columns 183; sixteen epilogue warps 191
-// (GELU 183). On random values the clock falls to 1.5 GHz at 1000 W, so energy a product decides there.
+// The epilogue's signals that an accumulator is free carry no release at cluster scope, which waited for its stores (a
+// tile took 1900 cycles longer: 162 instead of 138 us below).
+// Measured from 8-bit operands at the full clock (zeros): 17280 × 8960 × 1536 138 us = 3442 TFLOP/s, with GELU 149;
+// 17280 × 1536 × 8960 129 us = 3694. 4 stages 151, 150 and 148 us; groups of 8 tile rows 146, 152 and 130. On random
+// values the clock falls to 1.5 GHz at 1000 W and energy decides: 180 us = 2644 TFLOP/s, 195 and (gated) 183.
+// Not kept, measured before the two lines above held: 256 × 384 tiles in two accumulators of 192 columns, and sixteen
+// epilogue warps (each slower than 256 × 256 and eight, but GELU with sixteen).
 //
 // The tensor core adds to its fp32 accumulator by truncation, an error that grows with the number of additions (measured
 // relative to the result: 2e-7 after K = 4096, 1.3e-6 after 17280, on zero-mean operands; a bf16 output does not see it).
@@ -69,8 +72,8 @@ constexpr uint32_t kOffScale = kOffChunks + kEpiWarps * kChunkRoom;
 constexpr uint32_t kOffBar = kOffScale + kStages * kScaleBytes;
 constexpr uint32_t kOffTmemSlot = kOffBar + 8 * kNumBars;
 constexpr uint32_t kOffAbort = kOffTmemSlot + 4;
-constexpr uint32_t kOffCols = (kOffAbort + 4 + 15) & ~15u;  // bias[256], gate[256] as fp32
-constexpr uint32_t kSmemBytes = 1024 + kOffCols + 2 * kBN * 4;
+constexpr uint32_t kOffCols = (kOffAbort + 4 + 15) & ~15u;  // bias[256], gate[256] as fp32, of this tile and the next
+constexpr uint32_t kSmemBytes = 1024 + kOffCols + 4 * kBN * 4;
 static_assert(kSmemBytes <= 232448, "shared memory");
 
 struct Work {
@@ -213,8 +216,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const int quarter = warp & 3, half = (warp - 2) >> 2;
         const int et = threadIdx.x - 64;
         const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * (kBN / 2));
-        float* bias_s = reinterpret_cast<float*>(smem + kOffCols);
-        float* gate_s = bias_s + kBN;
+        // a thread's column of bias and gate, for the tile's 256 columns: fetched for the next tile under this one's work
+        float* const cols = reinterpret_cast<float*>(smem + kOffCols);
+        float next_bias = 0.0f, next_gate = 0.0f;
+        auto fetch_cols = [&](int t) {
+            int m0, n0, kb0, kb1;
+            place(t, m0, n0, kb0, kb1);
+            const int c = n0 + et;
+            next_bias = next_gate = 0.0f;
+            if (t < items && c < a.N) {
+                if (a.bias) next_bias = __bfloat162float(a.bias[c]);
+                if (kMode == FVSR_LINEAR_GATED_RESIDUAL) next_gate = __bfloat162float(a.gate[c]);
+            }
+        };
+        auto put_cols = [&](int buffer) {
+            cols[buffer * 2 * kBN + et] = next_bias;
+            if (kMode == FVSR_LINEAR_GATED_RESIDUAL) cols[buffer * 2 * kBN + kBN + et] = next_gate;
+        };
         const uint32_t acc_empty0 = mapa_shared(bar(kBarAccEmpty), 0), ovl0 = mapa_shared(bar(kBarOvl), 0);
         const bool leader = elect_one();  // issues the warp's copies and signals
         constexpr bool kBf16 = sizeof(T) == 2;
@@ -225,15 +243,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const uint32_t swizzle = (kBf16 ? (uint32_t)lane >> 1 & 3u : (uint32_t)lane & 7u) << 4;
         const int src_bar = kBarSrc + 2 * (warp - 2);
         uint32_t src_phase = 0;  // bit b: parity of the next wait on chunk place b
-        int lt = 0;
+        int lt = 0, buffer = 0;
         bool ok = true;
-        for (int t = pair; t < items; t += npairs) {
+        fetch_cols(pair);
+        put_cols(0);
+        for (int t = pair; t < items; t += npairs, buffer ^= 1) {
             int m0, n0, kb0, kb1;
             place(t, m0, n0, kb0, kb1);
-            named_barrier_sync(1, kEpiThreads);
-            bias_s[et] = a.bias && n0 + et < a.N ? __bfloat162float(a.bias[n0 + et]) : 0.0f;
-            gate_s[et] = kMode == FVSR_LINEAR_GATED_RESIDUAL && n0 + et < a.N ? __bfloat162float(a.gate[n0 + et]) : 0.0f;
-            named_barrier_sync(1, kEpiThreads);
+            named_barrier_sync(1, kEpiThreads);  // the tile's columns are there, the other buffer's are done with
+            const float *bias_s = cols + buffer * 2 * kBN, *gate_s = bias_s + kBN;
+            fetch_cols(t + npairs);
             const int row0 = m0 + 128 * (int)rank + quarter * 32, plane = t % wk.splits;
             const int c0 = n0 + half * (kBN / 2);
             const float *bcol = bias_s + half * (kBN / 2), *gcol = gate_s + half * (kBN / 2);
@@ -376,7 +395,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 if (half != acc) {  // this half held the shared columns: half 1 of accumulator 0, half 0 of accumulator 1
                     tc_fence_before();
                     __syncwarp();
-                    if (leader) mbar_arrive_cluster(ovl0);
+                    if (leader) mbar_arrive_remote(ovl0);
                 }
 #pragma unroll
                 for (int i = 0; i < kBN / 64; i += 2) {
@@ -387,12 +406,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     if (i + 2 == kBN / 64) {  // the accumulator is in registers
                         tc_fence_before();
                         __syncwarp();
-                        if (leader) mbar_arrive_cluster(acc_empty0 + 8u * (uint32_t)acc);
+                        if (leader) mbar_arrive_remote(acc_empty0 + 8u * (uint32_t)acc);
                     }
                     emit(vb, i + 1);
                     if (i + 2 < kBN / 64) tmem_ld_wait(va);
                 }
             }
+            put_cols(buffer ^ 1);
         }
         if (wk.tma && leader) bulk_wait<0>();
     }
