@@ -21,6 +21,7 @@ def _call(fvsr, name, good, **change):
 
 QUANT = dict(rows=5, cols=9, x=OK, dtype=1, square=0, q=OK, scale=OK, qt=OK, scale_t=OK, stream=None)
 DEQUANT = dict(rows=5, cols=9, q=OK, scale=OK, out=OK, dtype=1, stream=None)
+CODES = dict(rows=5, cols=9, scale=OK, out=OK, stream=None)
 LINEAR = dict(m=5, n=6, k=7, x=OK, x_scale=OK, w=OK, w_scale=OK, bias=OK, epilogue=2, gate=OK, resid=OK, out=OK,
               out_dtype=1, workspace=OK, workspace_bytes=BIG, stream=None)
 NORM = dict(m=5, c=6, x=OK, dtype=1, weight=OK, bias=OK, shift=OK, scale=OK, eps=1e-6, out=OK, mean=OK, rstd=OK,
@@ -36,6 +37,8 @@ REFUSED = [
     ("fvsr_quantize_fp8", QUANT, dict(q=None), 1, b"together"), ("fvsr_quantize_fp8", QUANT, dict(scale_t=None), 1, b"together"),
     ("fvsr_quantize_fp8", QUANT, dict(q=None, scale=None, qt=None, scale_t=None), 1, b"required"),
     ("fvsr_quantize_fp8", QUANT, dict(x=ODD8), 1, b"aligned"), ("fvsr_quantize_fp8", QUANT, dict(scale_t=ODD8), 1, b"aligned"),
+    ("fvsr_fp8_codes", CODES, dict(out=None), 1, b"required"), ("fvsr_fp8_codes", CODES, dict(scale=ODD8), 1, b"aligned"),
+    ("fvsr_fp8_codes", CODES, dict(cols=0), 1, b"cols"),
     ("fvsr_dequantize_fp8", DEQUANT, dict(out=None), 1, b"required"), ("fvsr_dequantize_fp8", DEQUANT, dict(out=ODD2), 1, b"aligned"),
     ("fvsr_dequantize_fp8", DEQUANT, dict(q=ODD8), 1, b"aligned"), ("fvsr_dequantize_fp8", DEQUANT, dict(dtype=-1), 1, b"dtype"),
     ("fvsr_linear_fp8", LINEAR, dict(m=-1), 1, b"m must be"), ("fvsr_linear_fp8", LINEAR, dict(n=0), 1, b"n and k"),

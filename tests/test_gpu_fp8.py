@@ -165,6 +165,49 @@ def test_linear_fp8_forms_agree_and_repeat(gpu, m, n, k):
     gpu.device_check()
 
 
+@pytest.mark.parametrize("m,n,k", [(5, 128, 256), (300, 512, 640), (2600, 1104, 8300)])
+def test_linear_fp8_into_an_output_off_the_16_byte_grid(gpu, m, n, k):
+    """out and resid that start two or four bytes past the grid are written element by element: the same bits."""
+    for dtype in (BF16, F32):
+        x, w8, _, _, bias, gate, g = _operands(gpu, m, n, k, "fp8", True, 5)
+        resid = torch.randn((m, n), generator=g, device="cuda").to(dtype)
+        want = gpu.linear_fp8(x, w8, bias, epilogue=2, gate=gate, resid=resid, out_dtype=dtype)
+        off = 2 if dtype == BF16 else 1
+        room, held = (torch.full((m * n + 64,), 7.0, dtype=dtype, device="cuda") for _ in range(2))
+        out, res = room[off:off + m * n].view(m, n), held[off:off + m * n].view(m, n)
+        res.copy_(resid)
+        gpu.linear_fp8(x, w8, bias, epilogue=2, gate=gate, resid=res, out=out)
+        assert torch.equal(out, want)
+        assert (room[:off] == 7.0).all() and (room[off + m * n:] == 7.0).all()
+    gpu.device_check()
+
+
+def test_host_threads_on_streams_of_their_own(gpu):
+    """Four host threads, each with a stream and operands of its own, at once: each gets what a call alone gives."""
+    import threading
+    jobs = [_operands(gpu, m, 700, 1500, "bf16", True, 50 + m)[:2] for m in (1, 40, 300, 600)]
+    want = [gpu.linear_fp8(*j) for j in jobs]
+    torch.cuda.synchronize()
+    errors = []
+
+    def work(i):
+        try:
+            st = torch.cuda.Stream()
+            got = [gpu.linear_fp8(*jobs[i], stream=st) for _ in range(20)]
+            st.synchronize()
+            assert all(torch.equal(t, want[i]) for t in got)
+        except BaseException as e:  # re-raised below
+            errors.append(e)
+
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join(60)
+    assert not errors, errors
+    gpu.device_check()
+
+
 def test_linear_fp8_accuracy_of_a_long_sum(gpu):
     """fp32 sums over a long K stay fp32: relative to the result's norm, K = 17280 random products summed in fp32 are
     off by about sqrt(K) roundings of the running sum at worst, sqrt(17280) 2^-24 = 8e-6; twice that is the bar (an

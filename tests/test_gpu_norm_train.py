@@ -159,6 +159,37 @@ def test_rows_without_spread_and_bad_rows(gpu):
         assert torch.isnan(gpu.layernorm_train(x, eps=0.0)[0][1]).all()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("c", [256, 1536, 1000])
+def test_tensors_off_the_16_byte_grid(gpu, c, dtype):
+    """Contiguous views that start one element into a buffer: the same values as aligned tensors, nothing written outside."""
+    m = 70
+    x, v, dy, _ = _case(m, c, dtype, True, True, 3)
+
+    def shifted(t):
+        room = torch.full((t.numel() + 2,), 3.0, dtype=t.dtype, device="cuda")
+        view = room[1:-1].view(t.shape)
+        view.copy_(t)
+        return room, view
+
+    out, mean, rstd = gpu.layernorm_train(x, **v)
+    xs, vs = shifted(x)[1], {k: shifted(t)[1] for k, t in v.items()}
+    room, o = shifted(torch.zeros_like(x))
+    got = gpu.layernorm_train(xs, **vs, out=o)
+    # sums over other lanes' shares: each off by fp32's bar of the forward test, then one rounding of the output's type
+    bar = 2.0 ** -6 if dtype == BF16 else 1e-5
+    assert (got[0].double() - out.double()).abs().max() <= bar * out.double().abs().max()
+    assert room[0] == 3.0 and room[-1] == 3.0
+    vs.pop("shift")
+    a = gpu.layernorm_backward(dy, x, mean, rstd, weight=v["weight"], bias=v["bias"], scale=v["scale"])
+    room, d = shifted(torch.zeros_like(x))
+    b = gpu.layernorm_backward(shifted(dy)[1], xs, shifted(mean)[1], shifted(rstd)[1], **vs, dx=d)
+    for k in a:
+        step = 2.0 ** -6 if k == "dx" and dtype == BF16 else 1e-4
+        assert (a[k].double() - b[k].double()).abs().max() <= step * a[k].double().abs().max(), k
+    assert room[0] == 3.0 and room[-1] == 3.0
+
+
 def test_no_rows(gpu):
     x = torch.empty((0, 300), dtype=BF16, device="cuda")
     s = torch.ones(300, dtype=BF16, device="cuda")
