@@ -6,7 +6,7 @@
 // fp32 throughout, one rounding of y and dx to the tensors' type.
 //
 // Both passes are bound by memory, x (and dy) read once and the result written once. A thread owns eight neighbouring
-// channels of every row it meets, so the vectors, and in the backward pass the sums A and B of those channels, stay in
+// channels (or twice eight) of every row it meets, so the vectors, and in the backward pass the sums A and B of those channels, stay in
 // its registers over all rows: tpr = ⌈c / 8⌉ threads, in whole warps, work on a row, kRows rows at once to share a
 // barrier; narrow rows put several such groups in a CTA. Rows are copied ahead into shared memory with cp.async, each
 // thread its own pieces (so that no barrier guards them), kStages sets of rows deep: what is in flight costs no
@@ -163,29 +163,41 @@ __device__ __forceinline__ float rsqrt_refined(float v) {
 }
 
 constexpr int kStages = 3;
-// Rows at once: forward four of bf16, two of fp32, backward two; one for more than kWideC channels, where a CTA's 1024
-// threads have 64 registers each. Threads that the kernels' registers let an SM hold: 768 of the forward pass (80
-// registers), 576 of the backward pass (112; 512 in CTAs of 256).
-constexpr int kWideC = 4096, kBackwardRows = 2, kForwardThreads = 768, kBackwardThreads = 576;
+// Of the backward pass: with three, fp32 rings of three CTAs do not fit an SM (17280 × 1536: 94 against 90 µs), and bf16
+// gains nothing by the third.
+constexpr int kBackwardStages = 2;
+// Rows at once: forward four of bf16, two of fp32, backward two; with two pieces a thread, forward two and one, backward
+// one. Threads that the kernels' registers let an SM hold: 768 of the forward pass (80 registers), 576 of the backward
+// pass (112; 512 in CTAs of 256).
+constexpr int kBackwardRows = 2, kForwardThreads = 768, kBackwardThreads = 576;
 
-template <typename T, bool kVec, int kRows, int kMaxThreads>
+// kP: pieces of eight channels a thread owns, tpr · 8 channels apart.
+template <typename T, bool kVec, int kRows, int kP, int kMaxThreads>
 __global__ void __launch_bounds__(kMaxThreads, kForwardThreads / kMaxThreads > 1 ? kForwardThreads / kMaxThreads : 1)
     norm_train_kernel(const NormTrainArgs a, int tpr) {
-    extern __shared__ uint4 ring[];  // [kStages][kRows][words][kMaxThreads]
+    extern __shared__ uint4 ring[];  // [kStages][kRows][kP][words][kMaxThreads]
     __shared__ alignas(16) float part[2][32 * kRows];
-    constexpr int W = Piece<T>::kWords, kRowWords = W * kMaxThreads;
-    const int groups = (int)blockDim.x / tpr, g = (int)threadIdx.x / tpr;
-    const int col = ((int)threadIdx.x % tpr) * 8, n = max(0, min(8, a.c - col)), warps = tpr >> 5, warp0 = g * warps;
+    constexpr int kPieceWords = Piece<T>::kWords * kMaxThreads, kRowWords = kP * kPieceWords;
+    const int groups = (int)blockDim.x / tpr, g = (int)threadIdx.x / tpr, warps = tpr >> 5, warp0 = g * warps;
+    const int col0 = ((int)threadIdx.x % tpr) * 8;
+    auto col = [&](int p) { return col0 + p * tpr * 8; };
+    int lens[kP];
+#pragma unroll
+    for (int p = 0; p < kP; ++p) lens[p] = max(0, min(8, a.c - col(p)));
+    auto len = [&](int p) { return lens[p]; };  // of piece p
     const int step = (int)gridDim.x * groups * kRows, row_first = ((int)blockIdx.x * groups + g) * kRows, m = (int)a.m;
     const int64_t c = a.c;
     const float inv_c = 1.0f / (float)a.c;
     int left = m - row_first;  // rows from the group's next ones to the end
     const T* x = static_cast<const T*>(a.x);
-    int64_t fetch_at = row_first * c + col;  // of the rows to fetch next
+    int64_t fetch_at = row_first * c + col0;  // of the rows to fetch next
     auto fetch = [&](uint4* to, int rows) {
 #pragma unroll
         for (int i = 0; i < kRows; ++i)
-            fetch8<T, kVec>(x + fetch_at + i * c, i < rows ? n : 0, to + i * kRowWords, kMaxThreads);
+#pragma unroll
+            for (int p = 0; p < kP; ++p)
+                fetch8<T, kVec>(x + fetch_at + i * c + p * tpr * 8, i < rows ? len(p) : 0,
+                                to + i * kRowWords + p * kPieceWords, kMaxThreads);
         copy_async_commit();
         fetch_at += step * c;
     };
@@ -193,62 +205,76 @@ __global__ void __launch_bounds__(kMaxThreads, kForwardThreads / kMaxThreads > 1
     uint4* const mine = ring + threadIdx.x;
 #pragma unroll
     for (int s = 0; s < kStages - 1; ++s) fetch(mine + s * kRows * kRowWords, left - s * step);
-    uint64_t gain[4], base[4];
+    uint64_t gain[kP][4], base[kP][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        float gv[2], bv[2];
+    for (int p = 0; p < kP; ++p)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const bool here = 2 * i + j < n;
-            const int at = here ? col + 2 * i + j : 0;
-            const float s1 = 1.0f + vec_or<T>(a.scale, at, 0.0f);
-            gv[j] = here ? s1 * vec_or<T>(a.weight, at, 1.0f) : 0.0f;
-            bv[j] = here ? fmaf(vec_or<T>(a.bias, at, 0.0f), s1, vec_or<T>(a.shift, at, 0.0f)) : 0.0f;
+        for (int i = 0; i < 4; ++i) {
+            float gv[2], bv[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const bool here = 2 * i + j < len(p);
+                const int at = here ? col(p) + 2 * i + j : 0;
+                const float s1 = 1.0f + vec_or<T>(a.scale, at, 0.0f);
+                gv[j] = here ? s1 * vec_or<T>(a.weight, at, 1.0f) : 0.0f;
+                bv[j] = here ? fmaf(vec_or<T>(a.bias, at, 0.0f), s1, vec_or<T>(a.shift, at, 0.0f)) : 0.0f;
+            }
+            gain[p][i] = f2(gv[0], gv[1]), base[p][i] = f2(bv[0], bv[1]);
         }
-        gain[i] = f2(gv[0], gv[1]), base[i] = f2(bv[0], bv[1]);
-    }
     int stage = 0;
     for (int cta_left = m - (int)blockIdx.x * groups * kRows; cta_left > 0; cta_left -= step, left -= step) {
         fetch(mine + (stage == 0 ? kStages - 1 : stage - 1) * kRows * kRowWords, left - (kStages - 1) * step);
         copy_async_wait<kStages - 1>();
         const uint4* now = mine + stage * kRows * kRowWords;
         float sum[kRows], sq[kRows];
-        uint64_t f[kRows][4];
+        uint64_t f[kRows][kP][4];
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
-            pairs(now + i * kRowWords, kMaxThreads, f[i], x);
-            sum[i] = pair_sum(fadd2(fadd2(f[i][0], f[i][1]), fadd2(f[i][2], f[i][3])));
+            sum[i] = 0.0f;
+#pragma unroll
+            for (int p = 0; p < kP; ++p) {
+                uint64_t(&v)[4] = f[i][p];
+                pairs(now + i * kRowWords + p * kPieceWords, kMaxThreads, v, x);
+                sum[i] += pair_sum(fadd2(fadd2(v[0], v[1]), fadd2(v[2], v[3])));
+            }
         }
         group_sum<kRows>(sum, part[0], warp0, warps);
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
             sum[i] *= inv_c;
             const uint64_t minus = f2(-sum[i], -sum[i]);
-            uint64_t q = 0;
+            sq[i] = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                f[i][j] = fadd2(f[i][j], minus);
-                uint64_t d = f[i][j];
-                if (!kVec && 2 * j + 1 >= n) {  // a piece that ends inside
-                    float lo, hi;
-                    uf2(d, lo, hi);
-                    d = f2(2 * j < n ? lo : 0.0f, 0.0f);
+            for (int p = 0; p < kP; ++p) {
+                uint64_t q = 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint64_t d = f[i][p][j] = fadd2(f[i][p][j], minus);
+                    if (!kVec && 2 * j + 1 >= len(p)) {  // a piece that ends inside
+                        float lo, hi;
+                        uf2(d, lo, hi);
+                        d = f2(2 * j < len(p) ? lo : 0.0f, 0.0f);
+                    }
+                    q = ffma2(d, d, q);
                 }
-                q = ffma2(d, d, q);
+                if (len(p) > 0) sq[i] += pair_sum(q);
             }
-            sq[i] = n > 0 ? pair_sum(q) : 0.0f;
         }
         group_sum<kRows>(sq, part[1], warp0, warps);
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
             if (i >= left) break;
             const float rstd = rsqrt_refined(fmaf(sq[i], inv_c, a.eps));
-            if (col == 0) a.mean[m - left + i] = sum[i], a.rstd[m - left + i] = rstd;
-            if (n == 0) continue;
+            if (col0 == 0) a.mean[m - left + i] = sum[i], a.rstd[m - left + i] = rstd;
             const uint64_t r2 = f2(rstd, rstd);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) f[i][j] = ffma2(fmul2(f[i][j], r2), gain[j], base[j]);
-            store8<kVec>(static_cast<T*>(a.out) + (int64_t)(m - left + i) * c + col, n, f[i]);
+            for (int p = 0; p < kP; ++p) {
+                if (len(p) == 0) continue;
+                uint64_t(&v)[4] = f[i][p];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = ffma2(fmul2(v[j], r2), gain[p][j], base[p][j]);
+                store8<kVec>(static_cast<T*>(a.out) + (int64_t)(m - left + i) * c + col(p), len(p), v);
+            }
         }
         stage = stage == kStages - 1 ? 0 : stage + 1;
     }
@@ -256,120 +282,148 @@ __global__ void __launch_bounds__(kMaxThreads, kForwardThreads / kMaxThreads > 1
 }
 
 // kHeld: x is the 8-bit form; a piece of it is 8 bytes.
-template <typename T, bool kHeld, bool kVec, int kRows, int kMaxThreads>
+template <typename T, bool kHeld, bool kVec, int kRows, int kP, int kMaxThreads>
 __global__ void __launch_bounds__(kMaxThreads, kBackwardThreads / kMaxThreads > 1 ? kBackwardThreads / kMaxThreads : 1)
     norm_backward_kernel(const NormTrainArgs a, int tpr) {
-    extern __shared__ uint4 ring[];  // [kStages][kRows][words of dy][kMaxThreads], then the same of x (8 bytes if held)
+    constexpr int kStages = kBackwardStages;
+    extern __shared__ uint4 ring[];  // [kStages][kRows][kP][words of dy][kMaxThreads], then the same of x (8 bytes if held)
     __shared__ alignas(16) float part[2][32 * 2 * kRows];
-    constexpr int W = Piece<T>::kWords, kRowWords = W * kMaxThreads;
-    const int groups = (int)blockDim.x / tpr, g = (int)threadIdx.x / tpr;
-    const int col = ((int)threadIdx.x % tpr) * 8, n = max(0, min(8, a.c - col)), warps = tpr >> 5, warp0 = g * warps;
+    constexpr int kPieceWords = Piece<T>::kWords * kMaxThreads, kRowWords = kP * kPieceWords;
+    const int groups = (int)blockDim.x / tpr, g = (int)threadIdx.x / tpr, warps = tpr >> 5, warp0 = g * warps;
+    const int col0 = ((int)threadIdx.x % tpr) * 8;
+    auto col = [&](int p) { return col0 + p * tpr * 8; };
+    int lens[kP];
+#pragma unroll
+    for (int p = 0; p < kP; ++p) lens[p] = max(0, min(8, a.c - col(p)));
+    auto len = [&](int p) { return lens[p]; };  // of piece p
     const int step = (int)gridDim.x * groups * kRows, row_first = ((int)blockIdx.x * groups + g) * kRows, m = (int)a.m;
     const int64_t c = a.c, ld = fp8_ld(a.c);
     const float inv_c = -1.0f / (float)a.c;
     int left = m - row_first;  // rows from the group's next ones to the end
     const T *dy = static_cast<const T*>(a.dy), *x = static_cast<const T*>(a.x);
     const uint8_t* x8 = static_cast<const uint8_t*>(a.x);
-    int64_t fetch_at = row_first * c + col, fetch_at8 = row_first * ld + col;  // of the rows to fetch next
+    int64_t fetch_at = row_first * c + col0, fetch_at8 = row_first * ld + col0;  // of the rows to fetch next
     uint4* const mine = ring + threadIdx.x;
     uint4* const mine_x = mine + kStages * kRows * kRowWords;
     uint2* const mine_x8 = reinterpret_cast<uint2*>(ring + kStages * kRows * kRowWords) + threadIdx.x;
     auto fetch = [&](int stage, int rows) {
 #pragma unroll
-        for (int i = 0; i < kRows; ++i) {
-            const int here = i < rows ? n : 0;
-            fetch8<T, kVec>(dy + fetch_at + i * c, here, mine + (stage * kRows + i) * kRowWords, kMaxThreads);
-            if constexpr (kHeld) {
-                uint2* to = mine_x8 + (stage * kRows + i) * kMaxThreads;
-                copy_async8(to, x8 + fetch_at8 + i * ld, here > 0);
-            } else {
-                fetch8<T, kVec>(x + fetch_at + i * c, here, mine_x + (stage * kRows + i) * kRowWords, kMaxThreads);
+        for (int i = 0; i < kRows; ++i)
+#pragma unroll
+            for (int p = 0; p < kP; ++p) {
+                const int here = i < rows ? len(p) : 0, piece = (stage * kRows + i) * kP + p;
+                fetch8<T, kVec>(dy + fetch_at + i * c + p * tpr * 8, here, mine + piece * kPieceWords, kMaxThreads);
+                if constexpr (kHeld)
+                    copy_async8(mine_x8 + piece * kMaxThreads, x8 + fetch_at8 + i * ld + p * tpr * 8, here > 0);
+                else
+                    fetch8<T, kVec>(x + fetch_at + i * c + p * tpr * 8, here, mine_x + piece * kPieceWords, kMaxThreads);
             }
-        }
         copy_async_commit();
         fetch_at += step * c;
         if (kHeld) fetch_at8 += step * ld;
     };
     // the rows' statistics (and codes) one step ahead, in registers; past the last row, that row's: its dy there is zero
     float next_mean[kRows], next_rstd[kRows];
-    uint32_t next_code[kRows];
-    const int tile_bytes = (int)fp8_scale_tiles(a.c) * 512, block = min(col, a.c - 1) >> 7;
-    const uint8_t* codes = kHeld ? a.x_scale + (block >> 2) * 512 + (block & 3) : nullptr;
+    uint32_t next_code[kRows][kP];
+    const int tile_bytes = (int)fp8_scale_tiles(a.c) * 512;
+    int code_at[kP];
+#pragma unroll
+    for (int p = 0; p < kP; ++p) {
+        const int block = min(col(p), a.c - 1) >> 7;
+        code_at[p] = (block >> 2) * 512 + (block & 3);
+    }
     auto fetch_row = [&](int rows) {
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
             const int r = min(m - rows + i, m - 1);
             next_mean[i] = a.mean[r], next_rstd[i] = a.rstd[r];
-            if (kHeld) next_code[i] = codes[(int64_t)(r >> 7) * tile_bytes + (r & 31) * 16 + ((r >> 5) & 3) * 4];
+#pragma unroll
+            for (int p = 0; p < kP; ++p)
+                if (kHeld)
+                    next_code[i][p] =
+                        a.x_scale[(int64_t)(r >> 7) * tile_bytes + (r & 31) * 16 + ((r >> 5) & 3) * 4 + code_at[p]];
         }
     };
     griddep_wait_then_release();
 #pragma unroll
     for (int s = 0; s < kStages - 1; ++s) fetch(s, left - s * step);
     fetch_row(left);
-    uint64_t gain[4], sum_a[4], sum_b[4];
+    uint64_t gain[kP][4], sum_a[kP][4], sum_b[kP][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        float gv[2];
+    for (int p = 0; p < kP; ++p)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const bool here = 2 * i + j < n;
-            const int at = here ? col + 2 * i + j : 0;
-            gv[j] = here ? (1.0f + vec_or<T>(a.scale, at, 0.0f)) * vec_or<T>(a.weight, at, 1.0f) : 0.0f;
+        for (int i = 0; i < 4; ++i) {
+            float gv[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const bool here = 2 * i + j < len(p);
+                const int at = here ? col(p) + 2 * i + j : 0;
+                gv[j] = here ? (1.0f + vec_or<T>(a.scale, at, 0.0f)) * vec_or<T>(a.weight, at, 1.0f) : 0.0f;
+            }
+            gain[p][i] = f2(gv[0], gv[1]);
+            sum_a[p][i] = sum_b[p][i] = 0;
         }
-        gain[i] = f2(gv[0], gv[1]);
-        sum_a[i] = sum_b[i] = 0;
-    }
     int stage = 0, flip = 0;
     for (int cta_left = m - (int)blockIdx.x * groups * kRows; cta_left > 0; cta_left -= step, left -= step, flip ^= 1) {
         fetch(stage == 0 ? kStages - 1 : stage - 1, left - (kStages - 1) * step);
         copy_async_wait<kStages - 1>();
-        uint64_t norm[kRows][4], grad[kRows][4];
+        uint64_t norm[kRows][kP][4], grad[kRows][kP][4];
         float rstd[kRows], s[2 * kRows];
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
             rstd[i] = next_rstd[i];
-            const uint64_t minus = f2(-next_mean[i], -next_mean[i]);
-            pairs(mine + (stage * kRows + i) * kRowWords, kMaxThreads, grad[i], dy);
-            if constexpr (kHeld) {
-                const uint2 u = mine_x8[(stage * kRows + i) * kMaxThreads];
-                const uint32_t two[4] = {u.x, u.x >> 16, u.y, u.y >> 16};
-                const float down = fp8_down(next_code[i]);
+            const uint64_t minus = f2(-next_mean[i], -next_mean[i]), r2 = f2(rstd[i], rstd[i]);
+            s[2 * i] = s[2 * i + 1] = 0.0f;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {  // the scaling is exact: one rounding, in the subtraction
-                    float lo, hi;
-                    fp8_unpack2(two[j], lo, hi);
-                    norm[i][j] = ffma2(f2(lo, hi), f2(down, down), minus);
+            for (int p = 0; p < kP; ++p) {
+                const int piece = (stage * kRows + i) * kP + p;
+                uint64_t(&n)[4] = norm[i][p];
+                uint64_t(&d)[4] = grad[i][p];
+                pairs(mine + piece * kPieceWords, kMaxThreads, d, dy);
+                if constexpr (kHeld) {
+                    const uint2 u = mine_x8[piece * kMaxThreads];
+                    const uint32_t two[4] = {u.x, u.x >> 16, u.y, u.y >> 16};
+                    const float down = fp8_down(next_code[i][p]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {  // the scaling is exact: one rounding, in the subtraction
+                        float lo, hi;
+                        fp8_unpack2(two[j], lo, hi);
+                        n[j] = ffma2(f2(lo, hi), f2(down, down), minus);
+                    }
+                } else {
+                    pairs(mine_x + piece * kPieceWords, kMaxThreads, n, dy);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) n[j] = fadd2(n[j], minus);
                 }
-            } else {
-                pairs(mine_x + (stage * kRows + i) * kRowWords, kMaxThreads, norm[i], dy);
+                uint64_t s1 = 0, s2 = 0;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) norm[i][j] = fadd2(norm[i][j], minus);
+                for (int j = 0; j < 4; ++j) {
+                    n[j] = fmul2(n[j], r2);
+                    sum_a[p][j] = ffma2(d[j], n[j], sum_a[p][j]);
+                    sum_b[p][j] = fadd2(sum_b[p][j], d[j]);
+                    d[j] = fmul2(d[j], gain[p][j]);
+                    s1 = fadd2(s1, d[j]);
+                    s2 = ffma2(d[j], n[j], s2);
+                }
+                s[2 * i] += pair_sum(s1);
+                if (len(p) > 0) s[2 * i + 1] += pair_sum(s2);
             }
-            const uint64_t r2 = f2(rstd[i], rstd[i]);
-            uint64_t s1 = 0, s2 = 0;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                norm[i][j] = fmul2(norm[i][j], r2);
-                sum_a[j] = ffma2(grad[i][j], norm[i][j], sum_a[j]);
-                sum_b[j] = fadd2(sum_b[j], grad[i][j]);
-                grad[i][j] = fmul2(grad[i][j], gain[j]);
-                s1 = fadd2(s1, grad[i][j]);
-                s2 = ffma2(grad[i][j], norm[i][j], s2);
-            }
-            s[2 * i] = pair_sum(s1), s[2 * i + 1] = n > 0 ? pair_sum(s2) : 0.0f;
         }
         fetch_row(left - step);
         group_sum<2 * kRows>(s, part[flip], warp0, warps);
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
-            if (i >= left || n == 0) break;
+            if (i >= left) break;
             const float c1 = s[2 * i] * inv_c, c2 = s[2 * i + 1] * inv_c;
             const uint64_t c1p = f2(c1, c1), c2p = f2(c2, c2), r2 = f2(rstd[i], rstd[i]);
-            uint64_t f[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) f[j] = fmul2(ffma2(norm[i][j], c2p, fadd2(grad[i][j], c1p)), r2);
-            store8<kVec>(static_cast<T*>(a.out) + (int64_t)(m - left + i) * c + col, n, f);
+            for (int p = 0; p < kP; ++p) {
+                if (len(p) == 0) continue;
+                uint64_t f[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) f[j] = fmul2(ffma2(norm[i][p][j], c2p, fadd2(grad[i][p][j], c1p)), r2);
+                store8<kVec>(static_cast<T*>(a.out) + (int64_t)(m - left + i) * c + col(p), len(p), f);
+            }
         }
         stage = stage == kStages - 1 ? 0 : stage + 1;
     }
@@ -377,34 +431,37 @@ __global__ void __launch_bounds__(kMaxThreads, kBackwardThreads / kMaxThreads > 
     // the CTA's sums: the groups' in order, through the ring
     if (groups > 1) {
         __syncthreads();
-        ulonglong2* const held = reinterpret_cast<ulonglong2*>(ring);
+        uint64_t* const held = reinterpret_cast<uint64_t*>(ring);  // [8 kP][kMaxThreads]
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            held[i * kMaxThreads + threadIdx.x] = make_ulonglong2(sum_a[2 * i], sum_a[2 * i + 1]);
-            held[(2 + i) * kMaxThreads + threadIdx.x] = make_ulonglong2(sum_b[2 * i], sum_b[2 * i + 1]);
-        }
-        __syncthreads();
-        for (int o = 1; g == 0 && o < groups; ++o) {
+        for (int p = 0; p < kP; ++p)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const ulonglong2 va = held[i * kMaxThreads + threadIdx.x + o * tpr];
-                const ulonglong2 vb = held[(2 + i) * kMaxThreads + threadIdx.x + o * tpr];
-                sum_a[2 * i] = fadd2(sum_a[2 * i], va.x), sum_a[2 * i + 1] = fadd2(sum_a[2 * i + 1], va.y);
-                sum_b[2 * i] = fadd2(sum_b[2 * i], vb.x), sum_b[2 * i + 1] = fadd2(sum_b[2 * i + 1], vb.y);
+            for (int i = 0; i < 4; ++i) {
+                held[(8 * p + i) * kMaxThreads + threadIdx.x] = sum_a[p][i];
+                held[(8 * p + 4 + i) * kMaxThreads + threadIdx.x] = sum_b[p][i];
             }
-        }
+        __syncthreads();
+        for (int o = 1; g == 0 && o < groups; ++o)
+#pragma unroll
+            for (int p = 0; p < kP; ++p)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    sum_a[p][i] = fadd2(sum_a[p][i], held[(8 * p + i) * kMaxThreads + threadIdx.x + o * tpr]);
+                    sum_b[p][i] = fadd2(sum_b[p][i], held[(8 * p + 4 + i) * kMaxThreads + threadIdx.x + o * tpr]);
+                }
         if (g != 0) return;
     }
-    float* to = a.partial + (int64_t)blockIdx.x * 2 * a.c + col;
+    float* to = a.partial + (int64_t)blockIdx.x * 2 * a.c;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        float av[2], bv[2];
-        uf2(sum_a[i], av[0], av[1]);
-        uf2(sum_b[i], bv[0], bv[1]);
+    for (int p = 0; p < kP; ++p)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-            if (2 * i + j < n) to[2 * i + j] = av[j], to[a.c + 2 * i + j] = bv[j];
-    }
+        for (int i = 0; i < 4; ++i) {
+            float av[2], bv[2];
+            uf2(sum_a[p][i], av[0], av[1]);
+            uf2(sum_b[p][i], bv[0], bv[1]);
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                if (2 * i + j < len(p)) to[col(p) + 2 * i + j] = av[j], to[a.c + col(p) + 2 * i + j] = bv[j];
+        }
 }
 
 // The CTAs' sums of eight channels (a 32-byte sector): 64 rows of eight threads take every 64th CTA's each, eight at a
@@ -445,17 +502,24 @@ __global__ void __launch_bounds__(512) norm_vectors_kernel(const NormTrainArgs a
     if (a.dshift) a.dshift[c] = vb;
 }
 
-// Threads of a row and of a CTA for c channels, and how many CTAs share an SM.
+// Pieces a thread owns, threads of a row and of a CTA for c channels, and how many CTAs share an SM. Two pieces from 4096
+// channels on: one piece would take CTAs of over 512 threads with 64 registers each.
 struct Shape {
-    int tpr, threads, groups;
-    explicit Shape(int c) : tpr(((c + 7) / 8 + 31) / 32 * 32), groups(tpr >= 256 ? 1 : 256 / tpr) { threads = tpr * groups; }
-    int most_threads() const { return threads <= 192 ? 192 : threads <= 256 ? 256 : threads <= 512 ? 512 : 1024; }
+    int pieces, tpr, threads, groups;
+    explicit Shape(int c, int wide) : pieces(c > wide ? 2 : 1) {
+        tpr = ((c + 8 * pieces - 1) / (8 * pieces) + 31) / 32 * 32;
+        groups = tpr >= 256 ? 1 : 256 / tpr;
+        threads = tpr * groups;
+    }
+    int most_threads() const { return threads <= 192 ? 192 : threads <= 256 ? 256 : 512; }
     int ctas(int64_t m, int rows, int sm_threads) const {
         const int64_t need = (m + groups * rows - 1) / (groups * rows);
         const int64_t most = (int64_t)sm_count() * (sm_threads > threads ? sm_threads / threads : 1);
         return (int)(need < most ? need : most);
     }
 };
+constexpr int kForwardWide = 4096, kBackwardWide = 4096;
+
 template <auto kernel>
 cudaError_t launch_ring(int ctas, const Shape& s, size_t ring_bytes, const NormTrainArgs& a, cudaStream_t st) {
     if (ring_bytes > 40 * 1024) {
@@ -465,33 +529,45 @@ cudaError_t launch_ring(int ctas, const Shape& s, size_t ring_bytes, const NormT
     return launch_pdl(kernel, dim3(ctas), dim3(s.threads), ring_bytes, st, a, s.tpr);
 }
 
+template <typename T, bool kVec, int kRows, int kP>
+cudaError_t train_pieces(const NormTrainArgs& a, const Shape& s, cudaStream_t st) {
+    const int ctas = s.ctas(a.m, kRows, kForwardThreads);
+    const size_t ring = (size_t)kStages * kRows * kP * s.most_threads() * 8 * sizeof(T);
+    switch (s.most_threads()) {
+        case 192: return launch_ring<norm_train_kernel<T, kVec, kRows, kP, 192>>(ctas, s, ring, a, st);
+        case 256: return launch_ring<norm_train_kernel<T, kVec, kRows, kP, 256>>(ctas, s, ring, a, st);
+        default: return launch_ring<norm_train_kernel<T, kVec, kRows, kP, 512>>(ctas, s, ring, a, st);
+    }
+}
+
 template <typename T, bool kVec>
 cudaError_t train(const NormTrainArgs& a, cudaStream_t st) {
     constexpr int kRows = sizeof(T) == 2 ? 4 : 2;
-    const Shape s(a.c);
-    const int rows = a.c > kWideC ? 1 : kRows, ctas = s.ctas(a.m, rows, kForwardThreads);
-    const size_t ring = (size_t)kStages * rows * s.most_threads() * 8 * sizeof(T);
-    if (s.threads <= 192) return launch_ring<norm_train_kernel<T, kVec, kRows, 192>>(ctas, s, ring, a, st);
-    if (s.threads <= 256) return launch_ring<norm_train_kernel<T, kVec, kRows, 256>>(ctas, s, ring, a, st);
-    if (a.c <= kWideC) return launch_ring<norm_train_kernel<T, kVec, kRows, 512>>(ctas, s, ring, a, st);
-    return launch_ring<norm_train_kernel<T, kVec, 1, 1024>>(ctas, s, ring, a, st);
+    const Shape s(a.c, kForwardWide);
+    return s.pieces == 1 ? train_pieces<T, kVec, kRows, 1>(a, s, st) : train_pieces<T, kVec, kRows / 2, 2>(a, s, st);
+}
+
+template <typename T, bool kHeld, bool kVec, int kRows, int kP>
+cudaError_t backward_pieces(const NormTrainArgs& a, const Shape& s, int ctas, cudaStream_t st) {
+    const size_t ring = (size_t)kBackwardStages * kRows * kP * s.most_threads() * 8 * (sizeof(T) + (kHeld ? 1 : sizeof(T)));
+    switch (s.most_threads()) {
+        case 192: return launch_ring<norm_backward_kernel<T, kHeld, kVec, kRows, kP, 192>>(ctas, s, ring, a, st);
+        case 256: return launch_ring<norm_backward_kernel<T, kHeld, kVec, kRows, kP, 256>>(ctas, s, ring, a, st);
+        default: return launch_ring<norm_backward_kernel<T, kHeld, kVec, kRows, kP, 512>>(ctas, s, ring, a, st);
+    }
 }
 
 template <typename T, bool kHeld, bool kVec>
 cudaError_t backward_rows(const NormTrainArgs& a, const Shape& s, int ctas, cudaStream_t st) {
-    constexpr int kRows = kBackwardRows;
-    const size_t ring = (size_t)kStages * (a.c > kWideC ? 1 : kRows) * s.most_threads() * 8 * (sizeof(T) + (kHeld ? 1 : sizeof(T)));
-    if (s.threads <= 192) return launch_ring<norm_backward_kernel<T, kHeld, kVec, kRows, 192>>(ctas, s, ring, a, st);
-    if (s.threads <= 256) return launch_ring<norm_backward_kernel<T, kHeld, kVec, kRows, 256>>(ctas, s, ring, a, st);
-    if (a.c <= kWideC) return launch_ring<norm_backward_kernel<T, kHeld, kVec, kRows, 512>>(ctas, s, ring, a, st);
-    return launch_ring<norm_backward_kernel<T, kHeld, kVec, 1, 1024>>(ctas, s, ring, a, st);
+    return s.pieces == 1 ? backward_pieces<T, kHeld, kVec, kBackwardRows, 1>(a, s, ctas, st)
+                         : backward_pieces<T, kHeld, kVec, 1, 2>(a, s, ctas, st);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 template <typename T>
 cudaError_t backward(const NormTrainArgs& a, cudaStream_t st) {
-    const Shape s(a.c);
+    const Shape s(a.c, kBackwardWide);
     const int ctas = norm_backward_ctas(a.m, a.c);
     cudaError_t e = cudaSuccess;
     if (ctas > 0) {
@@ -508,7 +584,8 @@ cudaError_t backward(const NormTrainArgs& a, cudaStream_t st) {
 }  // namespace
 
 int norm_backward_ctas(int64_t m, int c) {
-    return Shape(c).ctas(m, c > kWideC ? 1 : kBackwardRows, kBackwardThreads);
+    const Shape s(c, kBackwardWide);
+    return s.ctas(m, s.pieces == 1 ? kBackwardRows : 1, kBackwardThreads);
 }
 
 cudaError_t launch_layernorm_train(const NormTrainArgs& a, cudaStream_t st) {
