@@ -369,10 +369,11 @@ fvsr_status fvsr_dequantize_fp8(int64_t rows, int64_t cols, const void* q, const
  * transposed w), its weight gradient (the transposed forms of dy and x; out FVSR_F32) and the single token's (m = 1).
  * epilogue: fvsr_linear_epilogue, in fp32 with one rounding at the end: GELU(tanh) of the linear, or resid + gate *
  * linear. bias and gate (n) bf16 (bias may be NULL); out and resid (m, n) of out_dtype (resid may be out; else out
- * overlaps none of the inputs). Sums in fp32 (an fp32 output's in chains of 4096 products added with rounding; the tensor core's
- * own additions truncate). workspace: fvsr_linear_fp8_workspace_size bytes (may be 0), 16-byte aligned, for this call
- * alone until it is done. m, n, k at most 2^22, each tensor at most 2^40 bytes. 16-byte alignment for x, w and the
- * scales, 4-byte for out and resid, 2-byte for bias and gate. */
+ * overlaps none of the inputs). Sums in fp32; an fp32 output's in chains of 4096 products, added with rounding, since the
+ * tensor core's own additions truncate. The same bits each time.
+ * workspace: fvsr_linear_fp8_workspace_size bytes on the current device (may be 0), 16-byte aligned, for this call alone
+ * until it is done. m, n, k at most 2^22, each tensor at most 2^40 bytes. 16-byte alignment for x, w and the scales,
+ * 4-byte for out and resid, 2-byte for bias and gate. */
 fvsr_status fvsr_linear_fp8_workspace_size(int32_t m, int32_t n, int32_t k, int32_t x_is_fp8, size_t* bytes);
 fvsr_status fvsr_linear_fp8(int32_t m, int32_t n, int32_t k, const void* x, const void* x_scale, const void* w,
                             const void* w_scale, const void* bias, int32_t epilogue, const void* gate,

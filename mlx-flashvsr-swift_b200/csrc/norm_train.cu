@@ -13,6 +13,9 @@
 // registers. Arithmetic is on pairs (f32x2), without which the backward pass would be bound by issue slots. The variance
 // is taken about the mean in a second pass over the pieces. The vectors' gradients are summed per CTA over its rows,
 // then over the CTAs by a second kernel, both in a fixed order, so they do not depend on timing.
+// One B200, bf16 (share of the copy rate, 6533 GB/s): 17,280 × 1536 forward 22 µs (0.74), backward 37 (0.66), from the 8-bit
+// form 40; 30,720 × 1536 34 (0.85), 55 (0.78) and 60; 4096 × 8192 27, 54 and 56. What keeps the backward pass from
+// memory's rate is instructions: 152 for a thread's eight values of a row (194 from 8 bits).
 #include "../../include/fvsr_lcsa.h"
 #include "common.cuh"
 #include "fp8.cuh"
