@@ -505,11 +505,12 @@ __global__ void __launch_bounds__(512) norm_vectors_kernel(const NormTrainArgs a
     if (a.dshift) a.dshift[c] = vb;
 }
 
-// Pieces a thread owns, threads of a row and of a CTA for c channels, and how many CTAs share an SM. Two pieces from 4096
-// channels on: one piece would take CTAs of over 512 threads with 64 registers each.
+// Pieces a thread owns, threads of a row and of a CTA for c channels, and how many CTAs share an SM. Two pieces above
+// 4096 channels: one would take CTAs of over 512 threads with 64 registers each (4096 × 8192 bf16 forward 38 instead of 27
+// µs, backward 59 / 54); at 1536 two are slower (forward 24 / 22, backward 40 / 37).
 struct Shape {
     int pieces, tpr, threads, groups;
-    explicit Shape(int c, int wide) : pieces(c > wide ? 2 : 1) {
+    explicit Shape(int c) : pieces(c > 4096 ? 2 : 1) {
         tpr = ((c + 8 * pieces - 1) / (8 * pieces) + 31) / 32 * 32;
         groups = tpr >= 256 ? 1 : 256 / tpr;
         threads = tpr * groups;
@@ -521,7 +522,6 @@ struct Shape {
         return (int)(need < most ? need : most);
     }
 };
-constexpr int kForwardWide = 4096, kBackwardWide = 4096;
 
 template <auto kernel>
 cudaError_t launch_ring(int ctas, const Shape& s, size_t ring_bytes, const NormTrainArgs& a, cudaStream_t st) {
@@ -536,28 +536,28 @@ template <typename T, bool kVec, int kRows, int kP>
 cudaError_t train_pieces(const NormTrainArgs& a, const Shape& s, cudaStream_t st) {
     const int ctas = s.ctas(a.m, kRows, kForwardThreads);
     const size_t ring = (size_t)kStages * kRows * kP * s.most_threads() * 8 * sizeof(T);
-    switch (s.most_threads()) {
-        case 192: return launch_ring<norm_train_kernel<T, kVec, kRows, kP, 192>>(ctas, s, ring, a, st);
-        case 256: return launch_ring<norm_train_kernel<T, kVec, kRows, kP, 256>>(ctas, s, ring, a, st);
-        default: return launch_ring<norm_train_kernel<T, kVec, kRows, kP, 512>>(ctas, s, ring, a, st);
+    if constexpr (kP == 1) {  // two pieces: more than 256 threads
+        if (s.threads <= 192) return launch_ring<norm_train_kernel<T, kVec, kRows, kP, 192>>(ctas, s, ring, a, st);
+        if (s.threads <= 256) return launch_ring<norm_train_kernel<T, kVec, kRows, kP, 256>>(ctas, s, ring, a, st);
     }
+    return launch_ring<norm_train_kernel<T, kVec, kRows, kP, 512>>(ctas, s, ring, a, st);
 }
 
 template <typename T, bool kVec>
 cudaError_t train(const NormTrainArgs& a, cudaStream_t st) {
     constexpr int kRows = sizeof(T) == 2 ? 4 : 2;
-    const Shape s(a.c, kForwardWide);
+    const Shape s(a.c);
     return s.pieces == 1 ? train_pieces<T, kVec, kRows, 1>(a, s, st) : train_pieces<T, kVec, kRows / 2, 2>(a, s, st);
 }
 
 template <typename T, bool kHeld, bool kVec, int kRows, int kP>
 cudaError_t backward_pieces(const NormTrainArgs& a, const Shape& s, int ctas, cudaStream_t st) {
     const size_t ring = (size_t)kBackwardStages * kRows * kP * s.most_threads() * 8 * (sizeof(T) + (kHeld ? 1 : sizeof(T)));
-    switch (s.most_threads()) {
-        case 192: return launch_ring<norm_backward_kernel<T, kHeld, kVec, kRows, kP, 192>>(ctas, s, ring, a, st);
-        case 256: return launch_ring<norm_backward_kernel<T, kHeld, kVec, kRows, kP, 256>>(ctas, s, ring, a, st);
-        default: return launch_ring<norm_backward_kernel<T, kHeld, kVec, kRows, kP, 512>>(ctas, s, ring, a, st);
+    if constexpr (kP == 1) {  // two pieces: more than 256 threads
+        if (s.threads <= 192) return launch_ring<norm_backward_kernel<T, kHeld, kVec, kRows, kP, 192>>(ctas, s, ring, a, st);
+        if (s.threads <= 256) return launch_ring<norm_backward_kernel<T, kHeld, kVec, kRows, kP, 256>>(ctas, s, ring, a, st);
     }
+    return launch_ring<norm_backward_kernel<T, kHeld, kVec, kRows, kP, 512>>(ctas, s, ring, a, st);
 }
 
 template <typename T, bool kHeld, bool kVec>
@@ -570,7 +570,7 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 
 template <typename T>
 cudaError_t backward(const NormTrainArgs& a, cudaStream_t st) {
-    const Shape s(a.c, kBackwardWide);
+    const Shape s(a.c);
     const int ctas = norm_backward_ctas(a.m, a.c);
     cudaError_t e = cudaSuccess;
     if (ctas > 0) {
@@ -587,7 +587,7 @@ cudaError_t backward(const NormTrainArgs& a, cudaStream_t st) {
 }  // namespace
 
 int norm_backward_ctas(int64_t m, int c) {
-    const Shape s(c, kBackwardWide);
+    const Shape s(c);
     return s.ctas(m, s.pieces == 1 ? kBackwardRows : 1, kBackwardThreads);
 }
 
