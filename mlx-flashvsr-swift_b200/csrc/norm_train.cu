@@ -20,6 +20,7 @@
 #include "common.cuh"
 #include "fp8.cuh"
 #include "sm100.cuh"
+#include "unaligned.cuh"
 
 namespace fvsr {
 
@@ -42,81 +43,104 @@ __device__ __forceinline__ void copy_async_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
 }
 
-// Eight values of a row as stored: 16 bytes of bf16, 32 of fp32. In shared memory a piece is split into 16-byte words,
-// [word][thread], so that a warp's accesses are contiguous.
-template <typename T>
-struct Piece {
-    static constexpr int kWords = (int)sizeof(T) / 2;
-};
-
-// The piece of n (0 to 8) values at p into words w[0], w[stride], …: whole pieces (kVec: 16-byte aligned) asynchronously,
-// else element by element with zeros beyond n.
-template <typename T, bool kVec>
-__device__ __forceinline__ void fetch8(const T* p, int n, uint4* w, int stride) {
-    if constexpr (kVec) {
-#pragma unroll
-        for (int i = 0; i < Piece<T>::kWords; ++i)
-            copy_async16(w + i * stride, reinterpret_cast<const uint4*>(p) + i, n > 0);
-    } else {
-        alignas(16) T v[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : T(0.0f);
-#pragma unroll
-        for (int i = 0; i < Piece<T>::kWords; ++i) w[i * stride] = reinterpret_cast<const uint4*>(v)[i];
-    }
-}
-// A piece as four fp32 pairs.
 __device__ __forceinline__ uint64_t bf_pair(uint32_t u) {
     float lo, hi;
     bf2_to_f(u, lo, hi);
     return f2(lo, hi);
-}
-__device__ __forceinline__ void pairs(const uint4* w, int, uint64_t (&f)[4], const __nv_bfloat16*) {
-    const uint4 u = *w;
-    f[0] = bf_pair(u.x), f[1] = bf_pair(u.y), f[2] = bf_pair(u.z), f[3] = bf_pair(u.w);
-}
-__device__ __forceinline__ void pairs(const uint4* w, int stride, uint64_t (&f)[4], const float*) {
-    const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(w), b = *reinterpret_cast<const ulonglong2*>(w + stride);
-    f[0] = a.x, f[1] = a.y, f[2] = b.x, f[3] = b.y;
-}
-__device__ __forceinline__ uint32_t pack_pair(uint64_t v) {
-    float lo, hi;
-    uf2(v, lo, hi);
-    return pack_bf16x2(lo, hi);
 }
 __device__ __forceinline__ float pair_sum(uint64_t v) {
     float lo, hi;
     uf2(v, lo, hi);
     return lo + hi;
 }
-template <bool kVec>
-__device__ __forceinline__ void store8(__nv_bfloat16* p, int n, const uint64_t (&f)[4]) {
-    if (kVec) {
-        *reinterpret_cast<uint4*>(p) = make_uint4(pack_pair(f[0]), pack_pair(f[1]), pack_pair(f[2]), pack_pair(f[3]));
-    } else {
+__device__ __forceinline__ void to_regs(const uint4& u, uint32_t* v) { v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w; }
+// Zeros from value n on.
+__device__ __forceinline__ void clear_from(int n, uint64_t (&f)[4]) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            float v[2];
-            uf2(f[i >> 1], v[0], v[1]);
-            if (i < n) p[i] = __float2bfloat16_rn(v[i & 1]);
-        }
-    }
-}
-template <bool kVec>
-__device__ __forceinline__ void store8(float* p, int n, const uint64_t (&f)[4]) {
-    if (kVec) {
-        reinterpret_cast<ulonglong2*>(p)[0] = make_ulonglong2(f[0], f[1]);
-        reinterpret_cast<ulonglong2*>(p)[1] = make_ulonglong2(f[2], f[3]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            float v[2];
-            uf2(f[i >> 1], v[0], v[1]);
-            if (i < n) p[i] = v[i & 1];
-        }
+    for (int i = 0; i < 4; ++i) {
+        float lo, hi;
+        uf2(f[i], lo, hi);
+        f[i] = f2(2 * i < n ? lo : 0.0f, 2 * i + 1 < n ? hi : 0.0f);
     }
 }
 
+// Eight values of a row as stored: 16 bytes of bf16, 32 of fp32. In shared memory the pieces of kThreads threads take
+// kStride 16-byte words: if rows are 16-byte aligned and c a whole number of pieces (kVec), a piece's words are split,
+// [word][thread], so that a warp's accesses are contiguous; else each warp has its stretch of the row as the aligned words
+// that cover it, one more than its pieces have.
+template <typename T, bool kVec, int kThreads>
+struct Piece {
+    static constexpr int kWords = (int)sizeof(T) / 2, kRegs = kWords * 4;
+    static constexpr int kWarpStride = kVec ? 32 : kWords * 32 + 1, kStride = kWords * kThreads + (kVec ? 0 : kThreads / 32);
+
+    // Copies this thread's part of a row's piece, of which n values are there (n <= 0: zeros). p and to: kVec, its own
+    // piece; else its warp's, and the words may also hold what stands beside the row.
+    static __device__ __forceinline__ void fetch(const T* p, int n, uint4* to) {
+        if constexpr (kVec) {
+#pragma unroll
+            for (int i = 0; i < kWords; ++i)
+                copy_async16(to + i * kThreads, reinterpret_cast<const uint4*>(p) + i, n > 0);
+        } else {
+            const int lane = threadIdx.x & 31, off = (int)(reinterpret_cast<uintptr_t>(p) & 15);
+            const int bytes = n > 0 ? off + n * (int)sizeof(T) : 0;
+            const char* from = reinterpret_cast<const char*>(p) - off;
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) {
+                const int at = lane + 32 * i;
+                copy_async16(to + at, from + 16 * at, 16 * at < bytes);
+            }
+            if (lane == 0) copy_async16(to + 32 * kWords, from + 512 * kWords, 512 * kWords < bytes);
+        }
+    }
+    // This thread's piece as four fp32 pairs, zeros beyond its n values; off: the warp's p's offset from 16 bytes.
+    static __device__ __forceinline__ void read(const uint4* from, uint32_t off, int n, uint64_t (&f)[4]) {
+        uint32_t v[kRegs];
+        if constexpr (kVec) {
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) to_regs(from[i * kThreads], v + 4 * i);
+        } else {
+            uint32_t w[kRegs + 4];
+            from += (threadIdx.x & 31) * kWords;
+#pragma unroll
+            for (int i = 0; i <= kWords; ++i) to_regs(from[i], w + 4 * i);
+            shift_bytes<sizeof(T), kRegs>(w, off, v);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 2)
+                f[i] = bf_pair(v[i]);
+            else
+                f[i] = f2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+        }
+        if (!kVec && n < 8) clear_from(n, f);
+    }
+    // kVec: p is this thread's; else its warp's, which has n values.
+    static __device__ __forceinline__ void store(T* p, int n, const uint64_t (&f)[4]) {
+        uint32_t v[kRegs];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float lo, hi;
+            uf2(f[i], lo, hi);
+            if constexpr (sizeof(T) == 2)
+                v[i] = pack_bf16x2(lo, hi);
+            else
+                v[2 * i] = __float_as_uint(lo), v[2 * i + 1] = __float_as_uint(hi);
+        }
+        if constexpr (kVec) {
+#pragma unroll
+            for (int i = 0; i < kWords; ++i)
+                reinterpret_cast<uint4*>(p)[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        } else {
+            store_unaligned<T, kRegs>(p, n, v);
+        }
+    }
+};
+// The offset of row r from a 16-byte boundary, and so (pieces of a warp being whole multiples of 16 bytes apart) that of
+// its stretches.
+template <bool kVec, typename T>
+__device__ __forceinline__ uint32_t row_offset(const T* base, int r, int c) {
+    return kVec ? 0u : ((uint32_t)reinterpret_cast<uintptr_t>(base) + (uint32_t)r * (uint32_t)c * (uint32_t)sizeof(T)) & 15u;
+}
 template <typename T>
 __device__ __forceinline__ float vec_or(const void* v, int c, float otherwise) {
     return v ? load_as_float(static_cast<const T*>(v) + c) : otherwise;
@@ -180,7 +204,8 @@ __global__ void __launch_bounds__(kMaxThreads, kForwardThreads / kMaxThreads > 1
     norm_train_kernel(const NormTrainArgs a, int tpr) {
     extern __shared__ uint4 ring[];  // [kStages][kRows][kP][words][kMaxThreads]
     __shared__ alignas(16) float part[2][32 * kRows];
-    constexpr int kPieceWords = Piece<T>::kWords * kMaxThreads, kRowWords = kP * kPieceWords;
+    using P = Piece<T, kVec, kMaxThreads>;
+    constexpr int kPieceWords = P::kStride, kRowWords = kP * kPieceWords;
     const int groups = (int)blockDim.x / tpr, g = (int)threadIdx.x / tpr, warps = tpr >> 5, warp0 = g * warps;
     const int col0 = ((int)threadIdx.x % tpr) * 8;
     auto col = [&](int p) { return col0 + p * tpr * 8; };
@@ -188,24 +213,26 @@ __global__ void __launch_bounds__(kMaxThreads, kForwardThreads / kMaxThreads > 1
 #pragma unroll
     for (int p = 0; p < kP; ++p) lens[p] = max(0, min(8, a.c - col(p)));
     auto len = [&](int p) { return lens[p]; };  // of piece p
+    // where this thread's part in the copies starts, and how much of it a row has: its own pieces, or (not kVec) its warp's
+    const int at0 = kVec ? col0 : col0 & ~255;
+    auto here = [&](int p) { return kVec ? len(p) : min(256, a.c - at0 - p * tpr * 8); };
     const int step = (int)gridDim.x * groups * kRows, row_first = ((int)blockIdx.x * groups + g) * kRows, m = (int)a.m;
     const int64_t c = a.c;
     const float inv_c = 1.0f / (float)a.c;
     int left = m - row_first;  // rows from the group's next ones to the end
     const T* x = static_cast<const T*>(a.x);
-    int64_t fetch_at = row_first * c + col0;  // of the rows to fetch next
+    int64_t fetch_at = row_first * c + at0;  // of the rows to fetch next
     auto fetch = [&](uint4* to, int rows) {
 #pragma unroll
         for (int i = 0; i < kRows; ++i)
 #pragma unroll
             for (int p = 0; p < kP; ++p)
-                fetch8<T, kVec>(x + fetch_at + i * c + p * tpr * 8, i < rows ? len(p) : 0,
-                                to + i * kRowWords + p * kPieceWords, kMaxThreads);
+                P::fetch(x + fetch_at + i * c + p * tpr * 8, i < rows ? here(p) : 0, to + i * kRowWords + p * kPieceWords);
         copy_async_commit();
         fetch_at += step * c;
     };
     griddep_wait_then_release();
-    uint4* const mine = ring + threadIdx.x;
+    uint4* const mine = ring + (kVec ? (int)threadIdx.x : ((int)threadIdx.x >> 5) * P::kWarpStride);
 #pragma unroll
     for (int s = 0; s < kStages - 1; ++s) fetch(mine + s * kRows * kRowWords, left - s * step);
     uint64_t gain[kP][4], base[kP][4];
@@ -226,8 +253,10 @@ __global__ void __launch_bounds__(kMaxThreads, kForwardThreads / kMaxThreads > 1
         }
     int stage = 0;
     for (int cta_left = m - (int)blockIdx.x * groups * kRows; cta_left > 0; cta_left -= step, left -= step) {
+        if (!kVec) __syncwarp();  // the warp has read the stage that is filled now
         fetch(mine + (stage == 0 ? kStages - 1 : stage - 1) * kRows * kRowWords, left - (kStages - 1) * step);
         copy_async_wait<kStages - 1>();
+        if (!kVec) __syncwarp();  // and all its lanes' copies have arrived
         const uint4* now = mine + stage * kRows * kRowWords;
         float sum[kRows], sq[kRows];
         uint64_t f[kRows][kP][4];
@@ -237,7 +266,7 @@ __global__ void __launch_bounds__(kMaxThreads, kForwardThreads / kMaxThreads > 1
 #pragma unroll
             for (int p = 0; p < kP; ++p) {
                 uint64_t(&v)[4] = f[i][p];
-                pairs(now + i * kRowWords + p * kPieceWords, kMaxThreads, v, x);
+                P::read(now + i * kRowWords + p * kPieceWords, row_offset<kVec>(x, m - left + i, a.c), len(p), v);
                 sum[i] += pair_sum(fadd2(fadd2(v[0], v[1]), fadd2(v[2], v[3])));
             }
         }
@@ -272,11 +301,11 @@ __global__ void __launch_bounds__(kMaxThreads, kForwardThreads / kMaxThreads > 1
             const uint64_t r2 = f2(rstd, rstd);
 #pragma unroll
             for (int p = 0; p < kP; ++p) {
-                if (len(p) == 0) continue;
+                if (here(p) <= 0) continue;
                 uint64_t(&v)[4] = f[i][p];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) v[j] = ffma2(fmul2(v[j], r2), gain[p][j], base[p][j]);
-                store8<kVec>(static_cast<T*>(a.out) + (int64_t)(m - left + i) * c + col(p), len(p), v);
+                P::store(static_cast<T*>(a.out) + (int64_t)(m - left + i) * c + at0 + p * tpr * 8, here(p), v);
             }
         }
         stage = stage == kStages - 1 ? 0 : stage + 1;
@@ -291,7 +320,8 @@ __global__ void __launch_bounds__(kMaxThreads, kBackwardThreads / kMaxThreads > 
     constexpr int kStages = kBackwardStages;
     extern __shared__ uint4 ring[];  // [kStages][kRows][kP][words of dy][kMaxThreads], then the same of x (8 bytes if held)
     __shared__ alignas(16) float part[2][32 * 2 * kRows];
-    constexpr int kPieceWords = Piece<T>::kWords * kMaxThreads, kRowWords = kP * kPieceWords;
+    using P = Piece<T, kVec, kMaxThreads>;
+    constexpr int kPieceWords = P::kStride, kRowWords = kP * kPieceWords;
     const int groups = (int)blockDim.x / tpr, g = (int)threadIdx.x / tpr, warps = tpr >> 5, warp0 = g * warps;
     const int col0 = ((int)threadIdx.x % tpr) * 8;
     auto col = [&](int p) { return col0 + p * tpr * 8; };
@@ -299,14 +329,17 @@ __global__ void __launch_bounds__(kMaxThreads, kBackwardThreads / kMaxThreads > 
 #pragma unroll
     for (int p = 0; p < kP; ++p) lens[p] = max(0, min(8, a.c - col(p)));
     auto len = [&](int p) { return lens[p]; };  // of piece p
+    // where this thread's part in the copies starts, and how much of it a row has: its own pieces, or (not kVec) its warp's
+    const int at0 = kVec ? col0 : col0 & ~255;
+    auto here = [&](int p) { return kVec ? len(p) : min(256, a.c - at0 - p * tpr * 8); };
     const int step = (int)gridDim.x * groups * kRows, row_first = ((int)blockIdx.x * groups + g) * kRows, m = (int)a.m;
     const int64_t c = a.c, ld = fp8_ld(a.c);
     const float inv_c = -1.0f / (float)a.c;
     int left = m - row_first;  // rows from the group's next ones to the end
     const T *dy = static_cast<const T*>(a.dy), *x = static_cast<const T*>(a.x);
     const uint8_t* x8 = static_cast<const uint8_t*>(a.x);
-    int64_t fetch_at = row_first * c + col0, fetch_at8 = row_first * ld + col0;  // of the rows to fetch next
-    uint4* const mine = ring + threadIdx.x;
+    int64_t fetch_at = row_first * c + at0, fetch_at8 = row_first * ld + col0;  // of the rows to fetch next
+    uint4* const mine = ring + (kVec ? (int)threadIdx.x : ((int)threadIdx.x >> 5) * P::kWarpStride);
     uint4* const mine_x = mine + kStages * kRows * kRowWords;
     uint2* const mine_x8 = reinterpret_cast<uint2*>(ring + kStages * kRows * kRowWords) + threadIdx.x;
     auto fetch = [&](int stage, int rows) {
@@ -314,12 +347,12 @@ __global__ void __launch_bounds__(kMaxThreads, kBackwardThreads / kMaxThreads > 
         for (int i = 0; i < kRows; ++i)
 #pragma unroll
             for (int p = 0; p < kP; ++p) {
-                const int here = i < rows ? len(p) : 0, piece = (stage * kRows + i) * kP + p;
-                fetch8<T, kVec>(dy + fetch_at + i * c + p * tpr * 8, here, mine + piece * kPieceWords, kMaxThreads);
+                const int n = i < rows ? here(p) : 0, piece = (stage * kRows + i) * kP + p;
+                P::fetch(dy + fetch_at + i * c + p * tpr * 8, n, mine + piece * kPieceWords);
                 if constexpr (kHeld)
-                    copy_async8(mine_x8 + piece * kMaxThreads, x8 + fetch_at8 + i * ld + p * tpr * 8, here > 0);
+                    copy_async8(mine_x8 + piece * kMaxThreads, x8 + fetch_at8 + i * ld + p * tpr * 8, i < rows && len(p) > 0);
                 else
-                    fetch8<T, kVec>(x + fetch_at + i * c + p * tpr * 8, here, mine_x + piece * kPieceWords, kMaxThreads);
+                    P::fetch(x + fetch_at + i * c + p * tpr * 8, n, mine_x + piece * kPieceWords);
             }
         copy_async_commit();
         fetch_at += step * c;
@@ -368,8 +401,10 @@ __global__ void __launch_bounds__(kMaxThreads, kBackwardThreads / kMaxThreads > 
         }
     int stage = 0, flip = 0;
     for (int cta_left = m - (int)blockIdx.x * groups * kRows; cta_left > 0; cta_left -= step, left -= step, flip ^= 1) {
+        if (!kVec) __syncwarp();  // the warp has read the stage that is filled now
         fetch(stage == 0 ? kStages - 1 : stage - 1, left - (kStages - 1) * step);
         copy_async_wait<kStages - 1>();
+        if (!kVec) __syncwarp();  // and all its lanes' copies have arrived
         uint64_t norm[kRows][kP][4], grad[kRows][kP][4];
         float rstd[kRows], s[2 * kRows];
 #pragma unroll
@@ -382,7 +417,7 @@ __global__ void __launch_bounds__(kMaxThreads, kBackwardThreads / kMaxThreads > 
                 const int piece = (stage * kRows + i) * kP + p;
                 uint64_t(&n)[4] = norm[i][p];
                 uint64_t(&d)[4] = grad[i][p];
-                pairs(mine + piece * kPieceWords, kMaxThreads, d, dy);
+                P::read(mine + piece * kPieceWords, row_offset<kVec>(dy, m - left + i, a.c), len(p), d);
                 if constexpr (kHeld) {
                     const uint2 u = mine_x8[piece * kMaxThreads];
                     const uint32_t two[4] = {u.x, u.x >> 16, u.y, u.y >> 16};
@@ -394,7 +429,7 @@ __global__ void __launch_bounds__(kMaxThreads, kBackwardThreads / kMaxThreads > 
                         n[j] = ffma2(f2(lo, hi), f2(down, down), minus);
                     }
                 } else {
-                    pairs(mine_x + piece * kPieceWords, kMaxThreads, n, dy);
+                    P::read(mine_x + piece * kPieceWords, row_offset<kVec>(x, m - left + i, a.c), len(p), n);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) n[j] = fadd2(n[j], minus);
                 }
@@ -421,11 +456,11 @@ __global__ void __launch_bounds__(kMaxThreads, kBackwardThreads / kMaxThreads > 
             const uint64_t c1p = f2(c1, c1), c2p = f2(c2, c2), r2 = f2(rstd[i], rstd[i]);
 #pragma unroll
             for (int p = 0; p < kP; ++p) {
-                if (len(p) == 0) continue;
+                if (here(p) <= 0) continue;
                 uint64_t f[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) f[j] = fmul2(ffma2(norm[i][p][j], c2p, fadd2(grad[i][p][j], c1p)), r2);
-                store8<kVec>(static_cast<T*>(a.out) + (int64_t)(m - left + i) * c + col(p), len(p), f);
+                P::store(static_cast<T*>(a.out) + (int64_t)(m - left + i) * c + at0 + p * tpr * 8, here(p), f);
             }
         }
         stage = stage == kStages - 1 ? 0 : stage + 1;
@@ -515,7 +550,6 @@ struct Shape {
         groups = tpr >= 256 ? 1 : 256 / tpr;
         threads = tpr * groups;
     }
-    int most_threads() const { return threads <= 192 ? 192 : threads <= 256 ? 256 : 512; }
     int ctas(int64_t m, int rows, int sm_threads) const {
         const int64_t need = (m + groups * rows - 1) / (groups * rows);
         const int64_t most = (int64_t)sm_count() * (sm_threads > threads ? sm_threads / threads : 1);
@@ -532,15 +566,19 @@ cudaError_t launch_ring(int ctas, const Shape& s, size_t ring_bytes, const NormT
     return launch_pdl(kernel, dim3(ctas), dim3(s.threads), ring_bytes, st, a, s.tpr);
 }
 
+template <typename T, bool kVec, int kRows, int kP, int kMaxThreads>
+cudaError_t train_threads(const NormTrainArgs& a, const Shape& s, cudaStream_t st) {
+    const size_t ring = (size_t)16 * kStages * kRows * kP * Piece<T, kVec, kMaxThreads>::kStride;
+    return launch_ring<norm_train_kernel<T, kVec, kRows, kP, kMaxThreads>>(s.ctas(a.m, kRows, kForwardThreads), s, ring, a, st);
+}
+
 template <typename T, bool kVec, int kRows, int kP>
 cudaError_t train_pieces(const NormTrainArgs& a, const Shape& s, cudaStream_t st) {
-    const int ctas = s.ctas(a.m, kRows, kForwardThreads);
-    const size_t ring = (size_t)kStages * kRows * kP * s.most_threads() * 8 * sizeof(T);
     if constexpr (kP == 1) {  // two pieces: more than 256 threads
-        if (s.threads <= 192) return launch_ring<norm_train_kernel<T, kVec, kRows, kP, 192>>(ctas, s, ring, a, st);
-        if (s.threads <= 256) return launch_ring<norm_train_kernel<T, kVec, kRows, kP, 256>>(ctas, s, ring, a, st);
+        if (s.threads <= 192) return train_threads<T, kVec, kRows, kP, 192>(a, s, st);
+        if (s.threads <= 256) return train_threads<T, kVec, kRows, kP, 256>(a, s, st);
     }
-    return launch_ring<norm_train_kernel<T, kVec, kRows, kP, 512>>(ctas, s, ring, a, st);
+    return train_threads<T, kVec, kRows, kP, 512>(a, s, st);
 }
 
 template <typename T, bool kVec>
@@ -550,14 +588,20 @@ cudaError_t train(const NormTrainArgs& a, cudaStream_t st) {
     return s.pieces == 1 ? train_pieces<T, kVec, kRows, 1>(a, s, st) : train_pieces<T, kVec, kRows / 2, 2>(a, s, st);
 }
 
+template <typename T, bool kHeld, bool kVec, int kRows, int kP, int kMaxThreads>
+cudaError_t backward_threads(const NormTrainArgs& a, const Shape& s, int ctas, cudaStream_t st) {
+    constexpr int kDy = 16 * Piece<T, kVec, kMaxThreads>::kStride, kX = kHeld ? 8 * kMaxThreads : kDy;
+    const size_t ring = (size_t)kBackwardStages * kRows * kP * (kDy + kX);
+    return launch_ring<norm_backward_kernel<T, kHeld, kVec, kRows, kP, kMaxThreads>>(ctas, s, ring, a, st);
+}
+
 template <typename T, bool kHeld, bool kVec, int kRows, int kP>
 cudaError_t backward_pieces(const NormTrainArgs& a, const Shape& s, int ctas, cudaStream_t st) {
-    const size_t ring = (size_t)kBackwardStages * kRows * kP * s.most_threads() * 8 * (sizeof(T) + (kHeld ? 1 : sizeof(T)));
     if constexpr (kP == 1) {  // two pieces: more than 256 threads
-        if (s.threads <= 192) return launch_ring<norm_backward_kernel<T, kHeld, kVec, kRows, kP, 192>>(ctas, s, ring, a, st);
-        if (s.threads <= 256) return launch_ring<norm_backward_kernel<T, kHeld, kVec, kRows, kP, 256>>(ctas, s, ring, a, st);
+        if (s.threads <= 192) return backward_threads<T, kHeld, kVec, kRows, kP, 192>(a, s, ctas, st);
+        if (s.threads <= 256) return backward_threads<T, kHeld, kVec, kRows, kP, 256>(a, s, ctas, st);
     }
-    return launch_ring<norm_backward_kernel<T, kHeld, kVec, kRows, kP, 512>>(ctas, s, ring, a, st);
+    return backward_threads<T, kHeld, kVec, kRows, kP, 512>(a, s, ctas, st);
 }
 
 template <typename T, bool kHeld, bool kVec>
