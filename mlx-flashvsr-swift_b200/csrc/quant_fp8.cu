@@ -21,6 +21,7 @@
 #include "common.cuh"
 #include "fp8.cuh"
 #include "sm100.cuh"
+#include "unaligned.cuh"
 
 namespace fvsr {
 
@@ -294,7 +295,7 @@ __global__ void __launch_bounds__(kThreads) dequantize_kernel(int64_t rows, int6
 #pragma unroll
         for (int j = 0; j < kSteps; ++j) {
             const int at = j * 32 * kElems;
-            if (at >= left) break;
+            if (at >= left + (kVec ? 0 : lane * kElems)) break;  // else the whole warp's
             const int block = (lane * kElems + at) >> 7;
             const float down = fp8_down((word[i] >> (8 * block)) & 255u);
             const uint32_t w[2] = {reinterpret_cast<const uint32_t*>(&v[i][j])[0],
@@ -311,9 +312,11 @@ __global__ void __launch_bounds__(kThreads) dequantize_kernel(int64_t rows, int6
             } else if constexpr (kVec) {
                 *reinterpret_cast<float4*>(p + at) = make_float4(f[0], f[1], f[2], f[3]);
             } else {
+                uint32_t u[4];
 #pragma unroll
-                for (int e = 0; e < kElems; ++e)
-                    if (at + e < left) store_from_float(p + at + e, f[e]);
+                for (int e = 0; e < 4; ++e)
+                    u[e] = kElems == 8 ? pack_bf16x2(f[(2 * e) % kElems], f[(2 * e + 1) % kElems]) : __float_as_uint(f[e % kElems]);
+                store_unaligned<T, 4>(p - lane * kElems + at, min(32 * kElems, left + lane * kElems - at), u);
             }
         }
     }
