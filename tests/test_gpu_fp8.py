@@ -277,3 +277,20 @@ def test_two_streams_at_once(gpu):
     for i in range(2):
         assert all(torch.equal(t, want[i]) for t in got[i])
     gpu.device_check()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 5), (4, 8), (5, 127), (7, 131), (9, 511), (6, 513), (3, 1531), (2, 1536)])
+def test_dequantize_into_an_output_at_any_offset(gpu, rows, cols, dtype):
+    x8 = gpu.quantize_fp8(_x(rows, cols, dtype, rows + cols))
+    want = gpu.dequantize_fp8(x8, dtype=F32).to(dtype)
+    for off in range(9):
+        room = torch.full((rows * cols + 32,), 3.0, dtype=dtype, device="cuda")
+        out = room[8 + off:8 + off + rows * cols].view(rows, cols)
+        if out.data_ptr() % 4:
+            with pytest.raises(gpu.FVSRError, match="aligned"):
+                gpu.dequantize_fp8(x8, dtype=dtype, out=out)
+            continue
+        gpu.dequantize_fp8(x8, dtype=dtype, out=out)
+        assert torch.equal(out, want)
+        assert (room[:8 + off] == 3.0).all() and (room[8 + off + rows * cols:] == 3.0).all()

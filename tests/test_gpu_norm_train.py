@@ -267,3 +267,73 @@ def test_a_training_step_of_norm_and_linear_in_8_bits(gpu, m, c, n):
         a, b = got.double().flatten(), want.flatten()
         assert float(a @ b / (a.norm() * b.norm())) > 0.99
     gpu.device_check()
+
+
+def _placed(t, off, fill):
+    """t as a view that starts off elements past a 16-byte boundary, between elements of the value fill."""
+    room = torch.full((t.numel() + 32,), fill, dtype=t.dtype, device="cuda")
+    view = room[8 + off:8 + off + t.numel()].view(t.shape)
+    view.copy_(t)
+    return room, view
+
+
+def _untouched(room, off, n, fill):
+    return bool((room[:8 + off] == fill).all() and (room[8 + off + n:] == fill).all())
+
+
+PLACES = [(0, 0, 0), (1, 1, 1), (3, 3, 3), (1, 0, 2), (0, 3, 0)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("m,c", [(1, 3), (2, 7), (9, 8), (10, 257), (65, 130), (130, 12), (70, 1531), (33, 4095), (3, 4096),
+                                 (40, 4101), (5, 8185), (5, 8191), (3, 8192)])
+def test_rows_at_any_offset_between_values_that_are_not_theirs(gpu, m, c, dtype):
+    """Rows whose ends share 16-byte words with the next rows and with NaN before and behind the tensors, all tensors off
+    the grid alike or each by another amount: the formulas with the bars of the tests above, and nothing written outside."""
+    x, v, dy, _ = _case(m, c, dtype, True, True, 11 + m + c)
+    want, mean_w, rstd_w = ref.norm(x, **v)
+    xd = x.double()
+    size = xd.abs().mean(1)
+    n = (xd - mean_w[:, None]) * rstd_w[:, None]
+    rel = (D + 8) * U + (rstd_w * D * U * size) ** 2
+    e_n = rstd_w[:, None] * (D * U * size[:, None] + 2 * U * (xd - mean_w[:, None]).abs()) + rel[:, None] * n.abs()
+    w, b, s1, sh = _vec(v, x)
+    bar = (w * s1).abs() * e_n + 4 * U * ((n * w * s1).abs() + (b * s1).abs() + sh.abs())
+    vb = {k: t for k, t in v.items() if k != "shift"}
+    x8 = gpu.quantize_fp8(x)
+    for at_x, at_out, at_dy in PLACES:
+        xs, dys = _placed(x, at_x, float("nan"))[1], _placed(dy, at_dy, float("nan"))[1]
+        room, out = _placed(torch.zeros_like(x), at_out, 3.0)
+        _, mean, rstd = gpu.layernorm_train(xs, **v, out=out)
+        _within(mean, mean_w, D * U * size)
+        _within(rstd, rstd_w, rel * rstd_w)
+        _within(out, want, bar, dtype)
+        assert _untouched(room, at_out, x.numel(), 3.0)
+        for inp, values in ((xs, x), (x8, gpu.dequantize_fp8(x8, dtype=F32))):
+            room, dx = _placed(torch.zeros_like(x), at_out, 3.0)
+            got = gpu.layernorm_backward(dys, inp, mean, rstd, **vb, dx=dx)
+            assert got["dx"].data_ptr() == dx.data_ptr() and _untouched(room, at_out, x.numel(), 3.0)
+            bars = _backward_bars(dy, values, mean, rstd, vb)
+            for k, t in ref.norm_backward(dy, values, mean, rstd, **vb).items():
+                _within(got[k], t, bars[k], dtype if k == "dx" else F32)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("m,c", [(6, 5), (20, 129), (40, 1531), (12, 4099)])
+@pytest.mark.parametrize("off", [0, 1])
+def test_a_row_of_nan_leaves_its_neighbours(gpu, m, c, dtype, off):
+    x, v, dy, _ = _case(m, c, dtype, True, False, 12 + c)
+    out, mean, rstd = gpu.layernorm_train(x, **v)
+    x_bad, dy_bad = x.clone(), dy.clone()
+    x_bad[m // 2], dy_bad[m // 2] = float("nan"), float("inf")
+    bad = _placed(x_bad, off, 0.0)[1]
+    got, mean_b, rstd_b = gpu.layernorm_train(bad, **v, out=_placed(out, off, 0.0)[1])
+    rest = torch.arange(m, device="cuda") != m // 2
+    assert torch.equal(mean_b[rest].isnan().any(), torch.tensor(False, device="cuda")) and mean_b[~rest].isnan().all()
+    v.pop("shift"), v.pop("scale")
+    dx = gpu.layernorm_backward(dy, x, mean, rstd, **v)["dx"]
+    dx_b = gpu.layernorm_backward(_placed(dy_bad, off, 0.0)[1], bad, mean_b, rstd_b, **v, dx=_placed(dx, off, 0.0)[1])["dx"]
+    assert got[~rest].isnan().all() and dx_b[~rest].isnan().all()
+    if off == 0:  # the same rows in the same threads: the same bits
+        assert torch.equal(got[rest], out[rest]) and torch.equal(dx_b[rest], dx[rest])
+    assert torch.isfinite(got[rest]).all() and torch.isfinite(dx_b[rest]).all()
