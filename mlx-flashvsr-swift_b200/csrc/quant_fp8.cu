@@ -83,11 +83,24 @@ template <typename T>
 __device__ __forceinline__ int tile_word(int r, int w) {
     return r * Piece<T>::kLanes + (sizeof(T) == 2 ? w ^ ((r & 1) | (r >> 3 & 6)) : w);
 }
-// kVec: rows are 16-byte aligned and their lengths whole pieces; else element by element.
+// kVec: rows are 16-byte aligned and their lengths whole pieces; else bf16 from the one or two aligned words that hold the
+// piece, fp32 (whose pieces are four elements) element by element.
 template <typename T, bool kVec>
 __device__ __forceinline__ uint4 load_piece(const T* p, int left) {
     if constexpr (kVec) {
         return left > 0 ? __ldcs(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
+    } else if constexpr (sizeof(T) == 2) {
+        const uint32_t off = reinterpret_cast<uintptr_t>(p) & 15;
+        const uint4* from = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(p) - off);
+        const uint4 none = make_uint4(0, 0, 0, 0), a = left > 0 ? from[0] : none,
+                    b = (int)off + min(left, 8) * 2 > 16 ? from[1] : none;
+        uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}, o[4];
+        shift_bytes<2, 4>(w, off, o);
+        if (left < 8) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = 2 * i + 1 < left ? o[i] : 2 * i < left ? o[i] & 0xFFFFu : 0u;
+        }
+        return make_uint4(o[0], o[1], o[2], o[3]);
     } else {
         alignas(16) T v[Piece<T>::kElems];
 #pragma unroll
