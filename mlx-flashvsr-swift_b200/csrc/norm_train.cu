@@ -5,17 +5,25 @@
 //   A = Σ_rows dy·n, B = Σ_rows dy: dw = (1 + scale)·A, db = (1 + scale)·B, dscale = w·A + b·B, dshift = B.
 // fp32 throughout, one rounding of y and dx to the tensors' type.
 //
-// Both passes are bound by memory, x (and dy) read once and the result written once. A thread owns eight neighbouring
-// channels (or twice eight) of every row it meets, so the vectors, and in the backward pass the sums A and B of those channels, stay in
+// Both passes are bound by memory, x (and dy) read once and the result written once. A thread owns eight channels (or
+// twice eight) of every row it meets, so the vectors, and in the backward pass the sums A and B of those channels, stay in
 // its registers over all rows: tpr = ⌈c / 8⌉ threads, in whole warps, work on a row, kRows rows at once to share a
 // barrier; narrow rows put several such groups in a CTA. Rows are copied ahead into shared memory with cp.async, each
 // thread its own pieces (so that no barrier guards them), kStages sets of rows deep: what is in flight costs no
 // registers. Arithmetic is on pairs (f32x2), without which the backward pass would be bound by issue slots. The variance
 // is taken about the mean in a second pass over the pieces. The vectors' gradients are summed per CTA over its rows,
 // then over the CTAs by a second kernel, both in a fixed order, so they do not depend on timing.
-// One B200, bf16 (share of the copy rate, 6533 GB/s): 17,280 × 1536 forward 22 µs (0.74), backward 37 (0.66), from the 8-bit
-// form 40; 30,720 × 1536 34 (0.85), 55 (0.78) and 60; 4096 × 8192 27, 54 and 56. What keeps the backward pass from
-// memory's rate is instructions: 152 for a thread's eight values of a row (194 from 8 bits).
+// Where rows do not start on the 16-byte grid (c not a multiple of eight, or a tensor that starts off it) all accesses but
+// those at a row's two ends are still 16 aligned bytes (enum Grid below).
+// One B200, µs (share of the copy rate, 6533 GB/s):   forward     backward    from the 8-bit form
+//   17,280 × 1536 bf16                               22 (0.73)   37 (0.66)   40
+//   30,720 × 1536 bf16                               34 (0.84)   55 (0.79)   60
+//   4096 × 8192 bf16                                 28 (0.74)   54 (0.57)   56
+//   17,280 × 1536 fp32                               39 (0.83)   58 (0.85)   45
+//   17,280 × 1531 bf16                               33          46          67
+//   17,280 × 1531 fp32                               38          63          81
+// What keeps the backward pass in bf16 from memory's rate is instructions: 152 for a thread's eight values of a row (194
+// from 8 bits); off the grid the warps with a row's ends have the more of them that the row's other warps wait for.
 #include "../../include/fvsr_lcsa.h"
 #include "common.cuh"
 #include "fp8.cuh"
@@ -37,7 +45,8 @@ __device__ __forceinline__ void copy_async16(void* dst, const void* src, bool he
 }
 template <int kBytes>
 __device__ __forceinline__ void copy_async(void* dst, const void* src, bool here) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(smem_u32(dst)), "l"(src), "n"(kBytes), "r"(here ? kBytes : 0)
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(smem_u32(dst)), "l"(src), "n"(kBytes),
+                 "r"(here ? kBytes : 0)
                  : "memory");
 }
 template <int kParts>
@@ -83,8 +92,10 @@ __device__ __forceinline__ void clear_outside(const uint4* nibbles, uint32_t mas
 enum Grid {
     kWhole,    // rows start on it and are whole pieces
     kClasses,  // they do not, but all tensors' rows are off it alike: a group of threads keeps to rows that are off by the
-               // same, so its threads' pieces can start on the grid, the first before the row
-    kShifted,  // the tensors' rows are off it by different amounts: pieces start at the row's start and are shifted
+               // same, so its threads' pieces can start on the grid, the first before the row (17,280 × 1531 bf16 forward 33
+               // µs, element by element 68)
+    kShifted,  // the tensors' rows are off it by different amounts, or x is the 8-bit form, whose rows are never off it:
+               // pieces start at the row's start and are shifted (46 µs)
 };
 
 // A thread's eight values of a row: one 16-byte word of bf16, two of fp32, 32 words apart in the row, so that a warp's
@@ -162,7 +173,8 @@ struct Piece {
             for (int i = 0; i < kWords; ++i) {
                 const uint32_t in = of_word(part, i);
                 if (kGrid == kWhole ? in != 0 : in == (1 << kWord) - 1) {
-                    *reinterpret_cast<uint4*>(p + i * kNext) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                    *reinterpret_cast<uint4*>(p + i * kNext) =
+                        make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
                 } else if (kGrid == kClasses && in != 0) {
 #pragma unroll
                     for (int j = 0; j < kWord; ++j) {
@@ -192,11 +204,12 @@ struct Walk {
     __device__ __forceinline__ int row(int i) const { return cls + (i << log); }
 };
 
-// The offset of row r from a 16-byte boundary, and so (pieces of a warp being whole multiples of 16 bytes apart) that of
-// its stretches.
+// kShifted: the offset of row r from a 16-byte boundary, and so (a warp's stretches being whole multiples of 16 bytes
+// apart) that of its stretches.
 template <Grid kGrid, typename T>
 __device__ __forceinline__ uint32_t row_offset(const T* base, int r, int c) {
-    return kGrid != kShifted ? 0u : ((uint32_t)reinterpret_cast<uintptr_t>(base) + (uint32_t)r * (uint32_t)c * (uint32_t)sizeof(T)) & 15u;
+    if (kGrid != kShifted) return 0;
+    return ((uint32_t)reinterpret_cast<uintptr_t>(base) + (uint32_t)r * (uint32_t)c * (uint32_t)sizeof(T)) & 15u;
 }
 template <typename T>
 __device__ __forceinline__ float vec_or(const void* v, int c, float otherwise) {
@@ -247,8 +260,8 @@ __device__ __forceinline__ float rsqrt_refined(float v) {
 }
 
 constexpr int kStages = 3;
-// Of the backward pass: with three, fp32 rings of three CTAs do not fit an SM (17280 × 1536: 94 against 90 µs), and bf16
-// gains nothing by the third.
+// Of the backward pass: with three, fp32 rings of three CTAs do not fit an SM (17280 × 1536: 61 against 58 µs), and bf16
+// gains nothing by the third (37.3 / 36.7).
 constexpr int kBackwardStages = 2;
 // Rows at once: forward four of bf16, two of fp32, backward two; with two pieces a thread, forward two and one, backward
 // one. Threads that the kernels' registers let an SM hold: 768 of the forward pass (80 registers), 576 of the backward
@@ -269,7 +282,9 @@ __global__ void __launch_bounds__(kMaxThreads, kForwardThreads / kMaxThreads > 1
     const int low0 = kGrid == kClasses ? (int)((uint32_t)(reinterpret_cast<uintptr_t>(a.out) / sizeof(T)) +
                                                (uint32_t)walk.cls * (uint32_t)a.c) & (P::kWord - 1) : 0;
     const int at_warp = ((int)threadIdx.x % tpr & ~31) * 8 - low0, col0 = at_warp + ((int)threadIdx.x & 31) * P::kLane;
-    auto col = [&](int p, int j) { return col0 + p * tpr * 8 + j / P::kWord * P::kNext + j % P::kWord; };  // channel of value j
+    auto col = [&](int p, int j) {  // the channel of value j of piece p
+        return col0 + p * tpr * 8 + j / P::kWord * P::kNext + j % P::kWord;
+    };
     uint32_t mask[kP];
 #pragma unroll
     for (int p = 0; p < kP; ++p) {
@@ -291,7 +306,8 @@ __global__ void __launch_bounds__(kMaxThreads, kForwardThreads / kMaxThreads > 1
         for (int i = 0; i < kRows; ++i)
 #pragma unroll
             for (int p = 0; p < kP; ++p)
-                P::fetch(x + fetch_at + i * next + p * tpr * 8, i < rows ? there(p) : 0, to + i * kRowWords + p * kPieceWords);
+                P::fetch(x + fetch_at + i * next + p * tpr * 8, i < rows ? there(p) : 0,
+                         to + i * kRowWords + p * kPieceWords);
         copy_async_commit();
         fetch_at += step * next;
     };
@@ -393,7 +409,9 @@ __global__ void __launch_bounds__(kMaxThreads, kBackwardThreads / kMaxThreads > 
     const int low0 = kGrid == kClasses ? (int)((uint32_t)(reinterpret_cast<uintptr_t>(a.out) / sizeof(T)) +
                                                (uint32_t)walk.cls * (uint32_t)a.c) & (P::kWord - 1) : 0;
     const int at_warp = ((int)threadIdx.x % tpr & ~31) * 8 - low0, col0 = at_warp + ((int)threadIdx.x & 31) * P::kLane;
-    auto col = [&](int p, int j) { return col0 + p * tpr * 8 + j / P::kWord * P::kNext + j % P::kWord; };  // channel of value j
+    auto col = [&](int p, int j) {  // the channel of value j of piece p
+        return col0 + p * tpr * 8 + j / P::kWord * P::kNext + j % P::kWord;
+    };
     uint32_t mask[kP];
 #pragma unroll
     for (int p = 0; p < kP; ++p) {
@@ -455,7 +473,8 @@ __global__ void __launch_bounds__(kMaxThreads, kBackwardThreads / kMaxThreads > 
 #pragma unroll
             for (int p = 0; p < kP; ++p)
                 if (kHeld) {
-                    const uint8_t* code = a.x_scale + (int64_t)(r >> 7) * tile_bytes + (r & 31) * 16 + ((r >> 5) & 3) * 4 + code_at[p];
+                    const uint8_t* code =
+                        a.x_scale + (int64_t)(r >> 7) * tile_bytes + (r & 31) * 16 + ((r >> 5) & 3) * 4 + code_at[p];
                     next_code[i][p] = kParts == 1 ? *code : *reinterpret_cast<const uint16_t*>(code);
                 }
         }
@@ -620,7 +639,7 @@ __global__ void __launch_bounds__(512) norm_vectors_kernel(const NormTrainArgs a
 
 // Pieces a thread owns, threads of a row and of a CTA for c channels, and how many CTAs share an SM. Two pieces above
 // 4096 channels: one would take CTAs of over 512 threads with 64 registers each (4096 × 8192 bf16 forward 38 instead of 27
-// µs, backward 59 / 54); at 1536 two are slower (forward 24 / 22, backward 40 / 37).
+// µs, backward 59 / 54); below two are slower (1536: forward 26 / 22, backward 50 / 37; 4096: 33 / 32 and 52 / 49).
 struct Shape {
     int pieces, tpr, threads, groups, log_period;
     // word: values in 16 bytes. kClasses: up to word − 1 values more in front of a row, and rows are alike again after
