@@ -294,3 +294,25 @@ def test_dequantize_into_an_output_at_any_offset(gpu, rows, cols, dtype):
         gpu.dequantize_fp8(x8, dtype=dtype, out=out)
         assert torch.equal(out, want)
         assert (room[:8 + off] == 3.0).all() and (room[8 + off + rows * cols:] == 3.0).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("m,n,k", [(17, 1, 40), (40, 7, 130), (300, 129, 64), (257, 515, 200)])
+def test_a_residual_between_values_that_are_not_its_own(gpu, m, n, k, dtype):
+    """NaN before and behind a residual at each offset from the 16-byte grid that it may have (whole 4 bytes; others are
+    refused): the bits that it gives on the grid."""
+    g = torch.Generator(device="cuda").manual_seed(m + n)
+    x8, w8 = gpu.quantize_fp8(_x(m, k, BF16, 1)), gpu.quantize_fp8(_x(n, k, BF16, 2))
+    gate = torch.randn(n, generator=g, device="cuda").to(BF16)
+    resid = torch.randn((m, n), generator=g, device="cuda").to(dtype)
+    want = gpu.linear_fp8(x8, w8, epilogue=2, gate=gate, resid=resid, out_dtype=dtype)
+    assert torch.isfinite(want).all()
+    for off in (0, 1, 2, 4, 6) if dtype == BF16 else (0, 1, 3):
+        room = torch.full((m * n + 32,), float("nan"), dtype=dtype, device="cuda")
+        res = room[8 + off:8 + off + m * n].view(m, n)
+        res.copy_(resid)
+        if res.data_ptr() % 4:
+            with pytest.raises(gpu.FVSRError, match="aligned"):
+                gpu.linear_fp8(x8, w8, epilogue=2, gate=gate, resid=res, out_dtype=dtype)
+            continue
+        assert torch.equal(gpu.linear_fp8(x8, w8, epilogue=2, gate=gate, resid=res, out_dtype=dtype), want)
