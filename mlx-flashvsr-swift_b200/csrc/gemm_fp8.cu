@@ -554,8 +554,8 @@ cudaError_t launch_gemm_fp8(const Fp8GemmArgs& args, const Fp8GemmPlan& plan, fl
                 make_scale_map(&m.xs, args.x_scale, ((int64_t)args.M + 127) / 128 * kt4) &&
                 make_scale_map(&m.ws, args.w_scale, ((int64_t)args.N + 127) / 128 * kt4);
     m.out = m.resid = m.x;  // not used without tma
-    if (parts)
-        made = made && make_chunk_map(&m.out, partial, false, plan.splits, args.M, args.N, plan.partial_ld);
+    if (parts)  // with the rows' padding: the join reads it (beyond w's last row the products are zeros)
+        made = made && make_chunk_map(&m.out, partial, false, plan.splits, args.M, plan.partial_ld, plan.partial_ld);
     else if (wk.tma)
         made = made && make_chunk_map(&m.out, args.out, bf16, 1, args.M, args.N, args.N) &&
                (!gated || make_chunk_map(&m.resid, args.resid, bf16, 1, args.M, args.N, args.N));
