@@ -41,3 +41,20 @@ def test_a_sum_in_parts_does_not_depend_on_what_the_workspace_held(gpu, m, n, k,
     assert torch.isfinite(got[0]).all()
     assert all(torch.equal(t, got[0]) for t in got[1:])
     gpu.device_check()
+
+
+@pytest.mark.parametrize("m", [1, 9, 16, 17, 40, 300])
+def test_scales_that_meet_beyond_the_range_of_fp32(gpu, m):
+    """Operands of 2^118 and 2^-118: their products are ordinary numbers, their scales and the sums before scaling are not.
+    Bar: the sum's additions as in the linear layers' tests, (K + 8) 2^-23 sum|x w|, and the rounding of the output."""
+    n = 70
+    for k in (128, 700):
+        for e in (-118, -60, 60, 118):
+            x = (_rand(m + k, m, k) * 2.0 ** e).to(BF16)
+            x8, w8 = gpu.quantize_fp8(x), gpu.quantize_fp8(_rand(k, n, k) * 2.0 ** -e)
+            want, size = ref.linear(*(gpu.dequantize_fp8(t, dtype=F32).double() for t in (x8, w8)))
+            bar = (k + 8) * 2.0 ** -23 * size + 2.0 ** -24 * want.abs()
+            for inp in (x, x8):
+                d = (gpu.linear_fp8(inp, w8, out_dtype=F32).double() - want).abs()
+                assert (d <= bar).all(), (k, e, float((d / bar).max()))
+    gpu.device_check()
