@@ -807,6 +807,12 @@ def _channel_vector(t, name, n, dtype, like):
     return t.data_ptr()
 
 
+def _in_32_bits(*sizes) -> None:
+    """Refuses sizes that the C ABI's int32_t would take modulo 2^32."""
+    if max(sizes) > 0x7FFFFFFF:
+        raise FVSRError(FVSR_EUNSUPPORTED, f"a size of {max(sizes)} is too large")
+
+
 def _bytes(fn, device: int, *args) -> int:
     """A workspace size of the C ABI on the current device, remembered by its arguments."""
     key = (fn, device, args)
@@ -906,6 +912,7 @@ def linear_fp8(x, w: Fp8Tensor, bias=None, epilogue: int = FVSR_LINEAR, gate=Non
         with away:
             return linear_fp8(x, w, bias, epilogue, gate, resid, out, out_dtype, workspace)
     (m, k), n = x.shape if held else xt.shape, w.rows
+    _in_32_bits(m, n, k)
     if w.cols != k or n < 1 or w.data.get_device() != xt.get_device():
         raise FVSRError(FVSR_EINVAL, f"w must be (N, {k}) on {xt.device}, got {w.shape} on {w.device}")
     bias = _channel_vector(bias, "bias", n, torch.bfloat16, xt)
@@ -930,6 +937,7 @@ def linear_fp8(x, w: Fp8Tensor, bias=None, epilogue: int = FVSR_LINEAR, gate=Non
 
 def linear_fp8_workspace_size(m: int, n: int, k: int, x_is_fp8: bool) -> int:
     """Bytes of workspace of a linear_fp8 call on the current device."""
+    _in_32_bits(m, n, k)
     cuda = _torch().cuda
     return _bytes("fvsr_linear_fp8_workspace_size", cuda.current_device() if cuda.is_available() else -1, m, n, k,
                   1 if x_is_fp8 else 0)
@@ -945,6 +953,7 @@ def layernorm_train(x, weight=None, bias=None, shift=None, scale=None, eps: floa
         with away:
             return layernorm_train(x, weight, bias, shift, scale, eps, out)
     (m, c), dt, f32 = x.shape, x.dtype, _torch().float32
+    _in_32_bits(c)
     weight, bias = _channel_vector(weight, "weight", c, dt, x), _channel_vector(bias, "bias", c, dt, x)
     shift, scale = _channel_vector(shift, "shift", c, dt, x), _channel_vector(scale, "scale", c, dt, x)
     out = _torch().empty_like(x) if out is None else _matrix(out, "out", dtypes=(dt,), shape=x.shape, like=x)
@@ -965,6 +974,7 @@ def layernorm_backward(dy, x, mean, rstd, weight=None, bias=None, scale=None, dx
         with away:
             return layernorm_backward(dy, x, mean, rstd, weight, bias, scale, dx, workspace)
     (m, c), dt, f32 = dy.shape, dy.dtype, _torch().float32
+    _in_32_bits(c)
     if isinstance(x, Fp8Tensor):
         if x.shape != (m, c) or x.data.get_device() != dy.get_device():
             raise FVSRError(FVSR_EINVAL, f"x must be ({m}, {c}) on {dy.device}, got {x.shape} on {x.device}")

@@ -58,3 +58,18 @@ def test_scales_that_meet_beyond_the_range_of_fp32(gpu, m):
                 d = (gpu.linear_fp8(inp, w8, out_dtype=F32).double() - want).abs()
                 assert (d <= bar).all(), (k, e, float((d / bar).max()))
     gpu.device_check()
+
+
+def test_rows_and_channels_beyond_32_bits_are_refused(gpu):
+    """Not taken modulo 2^32, which gave the first 5 rows, or the statistics of the first 8 channels."""
+    rows = (1 << 32) + 5
+    x = torch.empty((rows, 1), dtype=BF16, device="cuda")
+    w8 = gpu.quantize_fp8(torch.ones((1, 1), device="cuda"))
+    with pytest.raises(gpu.FVSRError, match="too large"):
+        gpu.linear_fp8(x, w8)
+    x = x.view(-1)[:(1 << 32)].view(1, -1)
+    stat = torch.ones(1, device="cuda")
+    with pytest.raises(gpu.FVSRError, match="too large"):
+        gpu.layernorm_train(x)
+    with pytest.raises(gpu.FVSRError, match="too large"):
+        gpu.layernorm_backward(x, x, stat, stat)
