@@ -82,10 +82,11 @@ __device__ __forceinline__ void fill_nibbles(uint4* nibbles) {
         nibbles[t] = make_uint4(0u - (t & 1), 0u - (t >> 1 & 1), 0u - (t >> 2 & 1), 0u - (t >> 3 & 1));
     __syncthreads();
 }
-__device__ __forceinline__ void clear_outside(const uint4* nibbles, uint32_t mask, uint64_t (&f)[4]) {
+template <typename... Pieces>
+__device__ __forceinline__ void clear_outside(const uint4* nibbles, uint32_t mask, Pieces&... pieces) {
     const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(nibbles + (mask & 15));
     const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(nibbles + (mask >> 4));
-    f[0] &= a.x, f[1] &= a.y, f[2] &= b.x, f[3] &= b.y;
+    ((pieces[0] &= a.x, pieces[1] &= a.y, pieces[2] &= b.x, pieces[3] &= b.y), ...);
 }
 
 // How a row's pieces of eight values lie against the 16-byte grid.
@@ -131,9 +132,9 @@ struct Piece {
             for (int i = 0; i < kWords; ++i) copy_async16(to + i * kThreads, p + i * kNext, of_word(part, i) != 0);
         }
     }
-    // This thread's piece as four fp32 pairs, zeros outside the mask; off: the warp's p's offset from 16 bytes.
-    static __device__ __forceinline__ void read(const uint4* from, uint32_t off, uint32_t mask, const uint4* nibbles,
-                                                uint64_t (&f)[4]) {
+    // This thread's piece as four fp32 pairs, what is outside the mask as it stands there (zeros where it was not copied);
+    // off: the warp's p's offset from 16 bytes.
+    static __device__ __forceinline__ void read(const uint4* from, uint32_t off, uint64_t (&f)[4]) {
         uint32_t v[kRegs];
         if constexpr (kGrid == kShifted) {
             uint32_t w[kRegs + 4];
@@ -152,7 +153,10 @@ struct Piece {
             else
                 f[i] = f2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
         }
-        if (kGrid != kWhole && mask != 255) clear_outside(nibbles, mask, f);
+    }
+    template <typename... Pieces>
+    static __device__ __forceinline__ void clear(const uint4* nibbles, uint32_t mask, Pieces&... pieces) {
+        if (kGrid != kWhole && mask != 255) clear_outside(nibbles, mask, pieces...);
     }
     // p: as fetch.
     static __device__ __forceinline__ void store(T* p, int part, const uint64_t (&f)[4]) {
@@ -347,7 +351,8 @@ __global__ void __launch_bounds__(kMaxThreads, kForwardThreads / kMaxThreads > 1
 #pragma unroll
             for (int p = 0; p < kP; ++p) {
                 uint64_t(&v)[4] = f[i][p];
-                P::read(now + i * kRowWords + p * kPieceWords, row_offset<kGrid>(x, m - left + i, a.c), mask[p], nibbles, v);
+                P::read(now + i * kRowWords + p * kPieceWords, row_offset<kGrid>(x, m - left + i, a.c), v);
+                P::clear(nibbles, mask[p], v);
                 sum[i] += pair_sum(fadd2(fadd2(v[0], v[1]), fadd2(v[2], v[3])));
             }
         }
@@ -362,7 +367,7 @@ __global__ void __launch_bounds__(kMaxThreads, kForwardThreads / kMaxThreads > 1
                 uint64_t(&d)[4] = f[i][p];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) d[j] = fadd2(d[j], minus);
-                if (kGrid != kWhole && mask[p] != 255) clear_outside(nibbles, mask[p], d);
+                P::clear(nibbles, mask[p], d);
 #pragma unroll
                 for (int w = 0; w < P::kWords; ++w) {
                     uint64_t q = 0;
@@ -399,6 +404,9 @@ template <typename T, bool kHeld, Grid kGrid, int kRows, int kP, int kMaxThreads
 __global__ void __launch_bounds__(kMaxThreads, kBackwardThreads / kMaxThreads > 1 ? kBackwardThreads / kMaxThreads : 1)
     norm_backward_kernel(const NormTrainArgs a, int tpr, int log_period) {
     constexpr int kStages = kBackwardStages;
+    // dy's and n's values beside the row are cleared under one branch, but for two pieces of fp32 each, which spill so
+    // (4339 × 7415 off the grid by different amounts 119 µs instead of 108)
+    constexpr bool kOneClear = kHeld || kP * sizeof(T) < 8;
     extern __shared__ uint4 ring[];  // [kStages][kRows][kP][words of dy][kMaxThreads], then the same of x (8 bytes if held)
     __shared__ alignas(16) float part[2][32 * 2 * kRows];
     __shared__ uint4 nibbles[kGrid == kWhole ? 1 : 16];
@@ -455,7 +463,8 @@ __global__ void __launch_bounds__(kMaxThreads, kBackwardThreads / kMaxThreads > 
         fetch_at += step * next;
         if (kHeld) fetch_at8 += step * ld;
     };
-    // the rows' statistics (and codes) one step ahead, in registers; past the last row, that row's: its dy there is zero
+    // the rows' statistics (and codes) one step ahead, in registers; past the last row that row's, but rstd 0: n is zero there
+    // as dy is, where −mean · rstd may be infinite
     float next_mean[kRows], next_rstd[kRows];
     uint32_t next_code[kRows][kP];
     const int tile_bytes = (int)fp8_scale_tiles(a.c) * 512;
@@ -469,7 +478,7 @@ __global__ void __launch_bounds__(kMaxThreads, kBackwardThreads / kMaxThreads > 
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
             const int r = min(walk.row(m - rows + i), (int)a.m - 1);
-            next_mean[i] = a.mean[r], next_rstd[i] = a.rstd[r];
+            next_mean[i] = a.mean[r], next_rstd[i] = i < rows ? a.rstd[r] : 0.0f;
 #pragma unroll
             for (int p = 0; p < kP; ++p)
                 if (kHeld) {
@@ -517,7 +526,8 @@ __global__ void __launch_bounds__(kMaxThreads, kBackwardThreads / kMaxThreads > 
                 const int piece = (stage * kRows + i) * kP + p;
                 uint64_t(&n)[4] = norm[i][p];
                 uint64_t(&d)[4] = grad[i][p];
-                P::read(mine + piece * kPieceWords, row_offset<kGrid>(dy, m - left + i, a.c), mask[p], nibbles, d);
+                P::read(mine + piece * kPieceWords, row_offset<kGrid>(dy, m - left + i, a.c), d);
+                if constexpr (!kOneClear) P::clear(nibbles, mask[p], d);
                 if constexpr (kHeld) {
                     uint32_t u[2];
                     float down[2];
@@ -535,14 +545,21 @@ __global__ void __launch_bounds__(kMaxThreads, kBackwardThreads / kMaxThreads > 
                         n[j] = ffma2(f2(lo, hi), f2(down[j >> 1], down[j >> 1]), minus);
                     }
                 } else {
-                    P::read(mine_x + piece * kPieceWords, row_offset<kGrid>(x, m - left + i, a.c), mask[p], nibbles, n);
+                    P::read(mine_x + piece * kPieceWords, row_offset<kGrid>(x, m - left + i, a.c), n);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) n[j] = fadd2(n[j], minus);
                 }
+                // n after the subtraction: zero beside the row, not −mean · rstd
+                if constexpr (kOneClear)
+                    P::clear(nibbles, mask[p], d, n);
+                else
+                    P::clear(nibbles, mask[p], n);
                 uint64_t s1 = 0, s2 = 0;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    n[j] = fmul2(n[j], r2);
+                    // a word beside the row (bf16: the whole piece, below): n as P::clear leaves it
+                    const bool none = kGrid == kWhole && P::kWords == 2 && P::of_word(mask[p], 2 * j / P::kWord) == 0;
+                    n[j] = fmul2(n[j], none ? 0 : r2);
                     sum_a[p][j] = ffma2(d[j], n[j], sum_a[p][j]);
                     sum_b[p][j] = fadd2(sum_b[p][j], d[j]);
                     d[j] = fmul2(d[j], gain[p][j]);
@@ -550,7 +567,7 @@ __global__ void __launch_bounds__(kMaxThreads, kBackwardThreads / kMaxThreads > 
                     s2 = ffma2(d[j], n[j], s2);
                 }
                 s[2 * i] += pair_sum(s1);
-                if (mask[p] != 0) s[2 * i + 1] += pair_sum(s2);
+                if (kGrid != kWhole || P::kWords == 2 || mask[p] != 0) s[2 * i + 1] += pair_sum(s2);
             }
         }
         fetch_row(left - step);
