@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(kMaxThreads, kForwardThreads / kMaxThreads > 1
         for (int j = 0; j < 8; ++j) mask[p] |= (uint32_t)(0 <= col(p, j) && col(p, j) < a.c) << j;
     }
     // where this thread's part in the copies starts, and what a row has there (a piece's `part`)
-    const int at0 = kGrid == kShifted ? at_warp : col0;
+    const int at0 = kGrid == kShifted ? col0 & ~255 : col0;
     auto there = [&](int p) { return kGrid == kShifted ? min(256, a.c - at0 - p * tpr * 8) : (int)mask[p]; };
     const int step = walk.step, m = walk.m;  // in rows of the class
     const int64_t c = a.c, next = c << walk.log;  // from a row of the class to the next one
@@ -407,6 +407,9 @@ __global__ void __launch_bounds__(kMaxThreads, kBackwardThreads / kMaxThreads > 
     // dy's and n's values beside the row are cleared under one branch, but for two pieces of fp32 each, which spill so
     // (4339 × 7415 off the grid by different amounts 119 µs instead of 108)
     constexpr bool kOneClear = kHeld || kP * sizeof(T) < 8;
+    // What only the kernel's end needs is found anew there: kept, it is spilled in the loop (17,280 × 1531 bf16 from 8 bits 67
+    // instead of 66 µs, fp32 79 / 73; fp32 from fp32 is faster so, off the grid by different amounts 75 / 83).
+    constexpr bool kAnew = kGrid == kShifted && (kHeld || sizeof(T) == 2);
     extern __shared__ uint4 ring[];  // [kStages][kRows][kP][words of dy][kMaxThreads], then the same of x (8 bytes if held)
     __shared__ alignas(16) float part[2][32 * 2 * kRows];
     __shared__ uint4 nibbles[kGrid == kWhole ? 1 : 16];
@@ -428,7 +431,7 @@ __global__ void __launch_bounds__(kMaxThreads, kBackwardThreads / kMaxThreads > 
         for (int j = 0; j < 8; ++j) mask[p] |= (uint32_t)(0 <= col(p, j) && col(p, j) < a.c) << j;
     }
     // where this thread's part in the copies starts, and what a row has there (a piece's `part`)
-    const int at0 = kGrid == kShifted ? at_warp : col0;
+    const int at0 = kGrid == kShifted ? col0 & ~255 : col0;
     auto there = [&](int p) { return kGrid == kShifted ? min(256, a.c - at0 - p * tpr * 8) : (int)mask[p]; };
     const int step = walk.step, m = walk.m;  // in rows of the class
     const int64_t c = a.c, next = c << walk.log, ld = fp8_ld(a.c);  // next: from a row of the class to the next one
@@ -592,7 +595,10 @@ __global__ void __launch_bounds__(kMaxThreads, kBackwardThreads / kMaxThreads > 
     // the CTA's sums: its only group's, or the groups' in order, through the ring (by channel: the pieces of groups of
     // different classes lie differently)
     float* to = a.partial + (int64_t)blockIdx.x * 2 * a.c;
-    float* const own = groups > 1 ? reinterpret_cast<float*>(ring) + g * 2 * a.c : to;
+    int tid = threadIdx.x;
+    if constexpr (kAnew) asm volatile("" : "+r"(tid));  // not the tid that g, col0 and the masks are known for
+    float* const own = groups > 1 ? reinterpret_cast<float*>(ring) + tid / tpr * 2 * a.c : to;
+    auto end_col = [&](int p, int j) { return kAnew ? tid % tpr * 8 + p * tpr * 8 + j : col(p, j); };
     if (groups > 1) __syncthreads();
 #pragma unroll
     for (int p = 0; p < kP; ++p)
@@ -603,8 +609,8 @@ __global__ void __launch_bounds__(kMaxThreads, kBackwardThreads / kMaxThreads > 
             uf2(sum_b[p][i], bv[0], bv[1]);
 #pragma unroll
             for (int j = 0; j < 2; ++j)
-                if (mask[p] >> (2 * i + j) & 1)
-                    own[col(p, 2 * i + j)] = av[j], own[a.c + col(p, 2 * i + j)] = bv[j];
+                if (const int at = end_col(p, 2 * i + j); kAnew ? at < a.c : mask[p] >> (2 * i + j) & 1)
+                    own[at] = av[j], own[a.c + at] = bv[j];
         }
     if (groups == 1) return;
     __syncthreads();
