@@ -756,7 +756,7 @@ class Fp8Tensor:
     def codes(self, stream=None):
         """The blocks' codes in order (fvsr_fp8_codes), (rows, ceil(cols / 128)) uint8: a block's scale is
         2^(code - 127)."""
-        away = _elsewhere(self.scale, stream)
+        away = _elsewhere(self.scale, stream, self)
         if away is not None:
             with away:
                 return self.codes()
@@ -765,13 +765,18 @@ class Fp8Tensor:
         return out
 
 
-def _elsewhere(t, stream):
+def _elsewhere(t, stream, *used):
     """None when the current stream of the current device, t's, is where a call's launches and allocations belong; else
-    the context in which it is: memory allocated there belongs to the given stream."""
+    the context in which it is: memory allocated there belongs to the given stream, and that of `used` (tensors, 8-bit
+    tensors, None), which another stream may own, is not given away before the given stream is done with it."""
     torch = _torch()
     if stream is not None:
         if stream.device != t.device:
             raise FVSRError(FVSR_EINVAL, f"the stream is on {stream.device}, the tensors on {t.device}")
+        for u in used:
+            for part in (u.data, u.scale) if isinstance(u, Fp8Tensor) else (u,):
+                if part is not None and part.is_cuda:
+                    part.record_stream(stream)
         return torch.cuda.stream(stream)
     if torch._C._cuda_getDevice() != t.get_device():
         return torch.cuda.device(t.get_device())
@@ -845,7 +850,7 @@ def quantize_fp8(x, square: bool = False, transpose: bool = False, out=None, str
     128, or with square for each 128 x 128 square (weights). transpose: the form of x's transpose, (cols, rows), whose
     blocks run along x's rows (the checkpoint a weight gradient reads)."""
     x = _matrix(x, "x")
-    away = _elsewhere(x, stream)
+    away = _elsewhere(x, stream, x, out)
     if away is not None:
         with away:
             return quantize_fp8(x, square, transpose, out)
@@ -866,7 +871,7 @@ def quantize_fp8(x, square: bool = False, transpose: bool = False, out=None, str
 def quantize_fp8_both(x, square: bool = False, stream=None) -> tuple:
     """(quantize_fp8(x), quantize_fp8(x, transpose=True)) from one pass over x."""
     x = _matrix(x, "x")
-    away = _elsewhere(x, stream)
+    away = _elsewhere(x, stream, x)
     if away is not None:
         with away:
             return quantize_fp8_both(x, square)
@@ -881,7 +886,7 @@ def quantize_fp8_both(x, square: bool = False, stream=None) -> tuple:
 
 def dequantize_fp8(t: Fp8Tensor, dtype=None, out=None, stream=None):
     """The values of an 8-bit tensor as bf16 (the default) or fp32 (fvsr_dequantize_fp8)."""
-    away = _elsewhere(t.data, stream)
+    away = _elsewhere(t.data, stream, t, out)
     if away is not None:
         with away:
             return dequantize_fp8(t, dtype, out)
@@ -907,7 +912,7 @@ def linear_fp8(x, w: Fp8Tensor, bias=None, epilogue: int = FVSR_LINEAR, gate=Non
     xt = x.data if held else _matrix(x, "x", dtypes=(torch.bfloat16,))
     if not isinstance(w, Fp8Tensor):
         raise FVSRError(FVSR_EINVAL, "w must be an Fp8Tensor")
-    away = _elsewhere(xt, stream)
+    away = _elsewhere(xt, stream, x, w, bias, gate, resid, out, workspace)
     if away is not None:
         with away:
             return linear_fp8(x, w, bias, epilogue, gate, resid, out, out_dtype, workspace)
@@ -948,7 +953,7 @@ def layernorm_train(x, weight=None, bias=None, shift=None, scale=None, eps: floa
     out = (n * weight + bias) * (1 + scale) + shift; x (M, C) bf16 or fp32, the vectors (C) like x, mean and rstd (M)
     fp32 for layernorm_backward."""
     x = _matrix(x, "x")
-    away = _elsewhere(x, stream)
+    away = _elsewhere(x, stream, x, weight, bias, shift, scale, out)
     if away is not None:
         with away:
             return layernorm_train(x, weight, bias, shift, scale, eps, out)
@@ -969,7 +974,7 @@ def layernorm_backward(dy, x, mean, rstd, weight=None, bias=None, scale=None, dx
     8-bit form); weight, bias and scale as the forward had them. Returns {"dx", "dweight", "dbias", "dscale",
     "dshift"}: dx (M, C) like dy, the vectors' gradients (C) fp32, None where the forward had no such vector."""
     dy = _matrix(dy, "dy")
-    away = _elsewhere(dy, stream)
+    away = _elsewhere(dy, stream, dy, x, mean, rstd, weight, bias, scale, dx, workspace)
     if away is not None:
         with away:
             return layernorm_backward(dy, x, mean, rstd, weight, bias, scale, dx, workspace)

@@ -73,3 +73,42 @@ def test_rows_and_channels_beyond_32_bits_are_refused(gpu):
         gpu.layernorm_train(x)
     with pytest.raises(gpu.FVSRError, match="too large"):
         gpu.layernorm_backward(x, x, stat, stat)
+
+
+def test_temporaries_of_a_call_on_another_stream(gpu):
+    """Inputs that the caller lets go after a call on a stream that has not run yet: their memory is not given to the next
+    allocation of their own stream."""
+    x = _rand(1, 400, 512).to(BF16)
+    w8, v = gpu.quantize_fp8(_rand(2, 300, 512)), _rand(3, 512).to(BF16)
+    out, mean, rstd = gpu.layernorm_train(x, shift=v, scale=v)
+    calls = [
+        (lambda s, t: gpu.linear_fp8(t, w8, stream=s), lambda: x.clone()),
+        (lambda s, t: gpu.linear_fp8(t, w8, stream=s), lambda: gpu.quantize_fp8(x)),
+        (lambda s, t: gpu.linear_fp8(x, t, stream=s), lambda: gpu.quantize_fp8(_rand(2, 300, 512))),
+        (lambda s, t: gpu.quantize_fp8(t, stream=s).codes(), lambda: x.clone()),
+        (lambda s, t: gpu.dequantize_fp8(t, stream=s), lambda: gpu.quantize_fp8(x)),
+        (lambda s, t: gpu.layernorm_train(t, shift=v, scale=v, stream=s)[0], lambda: x.clone()),
+        (lambda s, t: gpu.layernorm_backward(t, x, mean, rstd, stream=s)["dx"], lambda: x.clone()),
+        (lambda s, t: gpu.layernorm_backward(x, t, mean, rstd, stream=s)["dx"], lambda: gpu.quantize_fp8(x)),
+    ]
+    side = torch.cuda.Stream()
+    for i, (call, make) in enumerate(calls):
+        want = call(None, make())
+        torch.cuda.synchronize()
+        t = make()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)
+        if i == 3:  # the codes are of the 8-bit tensor that the side stream fills
+            held = gpu.quantize_fp8(t, stream=side)
+            got = None
+        else:
+            got = call(side, t)
+        del t
+        junk = [torch.full((400, 512), float("nan"), device="cuda", dtype=BF16) for _ in range(4)]
+        junk += [torch.full((n, 512), 255, device="cuda", dtype=torch.uint8) for n in (400, 300, 400, 300, 4, 3, 4, 3)]
+        torch.cuda.synchronize()
+        got = held.codes() if got is None else got
+        assert torch.equal(got, want), i
+        del junk
+    gpu.device_check()
