@@ -369,8 +369,11 @@ fvsr_status fvsr_dequantize_fp8(int64_t rows, int64_t cols, const void* q, const
  * transposed w), its weight gradient (the transposed forms of dy and x; out FVSR_F32) and the single token's (m = 1).
  * epilogue: fvsr_linear_epilogue, in fp32 with one rounding at the end: GELU(tanh) of the linear, or resid + gate *
  * linear. bias and gate (n) bf16 (bias may be NULL); out and resid (m, n) of out_dtype (resid may be out; else out
- * overlaps none of the inputs). Sums in fp32; an fp32 output's in chains of 4096 products, added with rounding, since the
- * tensor core's own additions truncate. The same bits each time.
+ * overlaps none of the inputs). Sums in fp32. The tensor core's own additions truncate, so beyond 16 rows an fp32 output's
+ * sums are taken in chains of 4096 products, a bf16 output's in chains of 65536, added up with rounding: off by 2.3e-7 and
+ * 5e-6 of the result for operands of zero mean, by 1.5e-6 and 6e-5 for operands of one sign (measured). The same bits each
+ * time for the same shape and output type on the same device; a row's bits differ between calls of up to 16 rows and of
+ * more, and with the number of parts that m and n leave to the sum over k.
  * workspace: fvsr_linear_fp8_workspace_size bytes on the current device (may be 0), 16-byte aligned, for this call alone
  * until it is done. m, n, k at most 2^22, each tensor at most 2^40 bytes. 16-byte alignment for x, w and the scales,
  * 4-byte for out and resid, 2-byte for bias and gate. */

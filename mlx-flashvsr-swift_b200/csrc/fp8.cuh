@@ -109,7 +109,8 @@ struct Fp8GemmArgs {
     int mode, out_dtype;
 };
 // How a product is cut: `splits` parts of the sum over K, part_blocks blocks of 128 each (a multiple of 4: whole tiles of
-// codes) except the last; more than one part leaves fp32 partial products (splits, M, ld) in the workspace.
+// codes) except the last; more than one part, or a bf16 output's sum of more than one chain, leaves fp32 partial products
+// (splits, M, ld) in the workspace.
 struct Fp8GemmPlan {
     int splits, part_blocks;
     int64_t partial_ld;

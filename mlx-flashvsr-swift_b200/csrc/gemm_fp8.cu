@@ -32,10 +32,13 @@
 // Not kept, measured before the two lines above held: 256 × 384 tiles in two accumulators of 192 columns, and sixteen
 // epilogue warps (each slower than 256 × 256 and eight, but GELU with sixteen).
 //
-// The tensor core adds to its fp32 accumulator by truncation, an error that grows with the number of additions (measured
-// relative to the result: 2e-7 after K = 4096, 1.3e-6 after 17280, on zero-mean operands; a bf16 output does not see it).
-// For an fp32 output the sum is therefore taken in chains of 4096, which the epilogue adds up with rounding, in the
-// output itself: the accumulators alternate between chains as between tiles.
+// The tensor core adds to its fp32 accumulator by truncation, an error that grows with the number of additions and, where
+// the products have one sign, is a bias. Measured in one chain, relative to the result, zero-mean / one-signed operands:
+// K = 4096 2.2e-7 / 1.5e-6, 8960 6e-7 / 4.4e-6, 17280 1.3e-6 / 1.1e-5, 65536 5e-6 / 6e-5, 262144 4.3e-5 / 4.2e-4 (sums that
+// round, in torch: 8e-8 / 2.3e-7 at 4096). For an fp32 output the sum is therefore taken in chains of 4096, which the
+// epilogue adds up with rounding, in the output itself (2.3e-7 / 1.5e-6 whatever K): the accumulators alternate between
+// chains as between tiles. A bf16 output, whose rounding is 3.9e-3, is one chain up to 65536 (1/64 of that); beyond, its
+// chains are added up in an fp32 plane of the workspace, as the partial sums below are.
 // When the tiles are fewer than half the pairs, the sum over K is cut into parts (whole tiles of codes, 512 wide) that
 // leave fp32 partial products; a second kernel adds them in order and applies the epilogue.
 // Every wait is bounded (4 s); on expiry the kernel raises its abort and device timeout words, skips the rest of its
@@ -61,7 +64,7 @@ constexpr uint32_t kStageBytes = 2 * kHalfBytes;
 constexpr uint32_t kScaleBytes = 3 * 512;        // x's 128 rows, w's 256 rows, four blocks
 constexpr int kThreads = 320;
 constexpr int kEpiWarps = 8, kEpiThreads = 32 * kEpiWarps;
-constexpr int kChainBlocks = 32;                 // of 128: the longest chain of an fp32 output
+constexpr int kChainBlocks = 32, kLongChainBlocks = 512;  // of 128: the longest chains of an fp32 and of a bf16 output
 constexpr uint64_t kWaitLimitNs = 4000000000ull;
 constexpr uint32_t kIdesc = idesc_mxf8(kBM, kBN);
 constexpr uint32_t kAcc1 = 240, kTmemScale = 496;
@@ -530,7 +533,7 @@ Fp8GemmPlan plan_gemm_fp8(int M, int N, int K) {
     const int per = (groups + splits - 1) / splits;
     p.splits = (groups + per - 1) / per;
     p.part_blocks = 4 * per;
-    if (p.splits > 1) {
+    if (p.splits > 1 || kt > kLongChainBlocks) {
         p.partial_ld = (N + 3) / 4 * 4;  // 16-byte rows
         p.partial_bytes = (size_t)p.splits * M * p.partial_ld * sizeof(float);
     }
@@ -538,14 +541,15 @@ Fp8GemmPlan plan_gemm_fp8(int M, int N, int K) {
 }
 
 cudaError_t launch_gemm_fp8(const Fp8GemmArgs& args, const Fp8GemmPlan& plan, float* partial, cudaStream_t st) {
-    const bool parts = plan.splits > 1, bf16 = args.out_dtype == FVSR_BF16;
+    const bool bf16 = args.out_dtype == FVSR_BF16;
     Work wk;
     wk.mt = (args.M + kBM - 1) / kBM;
     wk.nt = (args.N + kBN - 1) / kBN;
     wk.kt = (args.K + kBK - 1) / kBK;
     wk.splits = plan.splits;
     wk.part_blocks = plan.part_blocks;
-    wk.chain_blocks = bf16 ? plan.part_blocks : kChainBlocks;
+    wk.chain_blocks = bf16 ? kLongChainBlocks : kChainBlocks;
+    const bool parts = plan.splits > 1 || (bf16 && wk.kt > kLongChainBlocks);  // by way of the workspace
     const bool gated = args.mode == FVSR_LINEAR_GATED_RESIDUAL;
     wk.tma = parts || ((int64_t)args.N * (bf16 ? 2 : 4) % 16 == 0 && aligned16(args.out) && (!gated || aligned16(args.resid)));
     Maps m;

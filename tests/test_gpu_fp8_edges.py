@@ -112,3 +112,61 @@ def test_temporaries_of_a_call_on_another_stream(gpu):
         assert torch.equal(got, want), i
         del junk
     gpu.device_check()
+
+
+def _products(gpu, m, n, k, one_sign):
+    """8-bit operands (m, k), (n, k) of random values, or of their magnitudes, and their product in 64 bits."""
+    x, w = _rand(m + k, m, k), _rand(n + k + 1, n, k)
+    x8, w8 = gpu.quantize_fp8(x.abs_() if one_sign else x), gpu.quantize_fp8(w.abs_() if one_sign else w)
+    xv, wv = (gpu.dequantize_fp8(t, dtype=F32, out=o) for t, o in ((x8, x), (w8, w)))
+    want = torch.zeros((m, n), dtype=torch.float64, device="cuda")
+    for at in range(0, k, 1 << 15):
+        want += xv[:, at:at + (1 << 15)].double() @ wv[:, at:at + (1 << 15)].double().t()
+    return x8, w8, want
+
+
+# An addition of 32 products truncates by at most 2^-23 of the running sum, which products of one sign let grow evenly: a chain
+# of c additions is off by at most (c + 1) / 2 * 2^-23 of its sum. In chains of 4096 (c = 128) that is 64.5 * 2^-23 = 7.7e-6,
+# and each addition of chains rounds by half of that step; one chain of 17280 was measured at 1.1e-5.
+SIGNED = 64.5 * 2.0 ** -23
+LONG = [(1280, 2048, 17280), (1280, 2046, 17280), (1280, 2047, 17280),  # not cut: chains in the output, on and off the grid
+        (1536, 1536, 34560), (1280, 1533, 34560)]                        # in two parts: chains in the planes of partial sums
+
+
+@pytest.mark.parametrize("m,n,k", LONG)
+def test_long_fp32_sums_are_taken_in_chains(gpu, m, n, k):
+    """One sign: each value within the bar above. Zero mean: relative to the result's norm, a chain of 4096 was measured at
+    2.2e-7 and one of 17280 at 1.3e-6; 6e-7 tells them apart."""
+    x8, w8, want = _products(gpu, m, n, k, True)
+    got = gpu.linear_fp8(x8, w8, out_dtype=F32).double()
+    bar = SIGNED + (k // 4096 + 2) * 2.0 ** -24
+    assert float(((got - want).abs() / want).max()) <= bar
+    # in place, gated: resid + gate * (x w), the gate a power of two, the residual about the sum's size
+    gate = torch.full((n,), 0.5, dtype=BF16, device="cuda")
+    resid = want.to(F32).clone()
+    start = resid.double() + 0.5 * want
+    out = gpu.linear_fp8(x8, w8, epilogue=2, gate=gate, resid=resid, out=resid)
+    assert out.data_ptr() == resid.data_ptr()
+    assert float(((out.double() - start).abs() / start).max()) <= bar + (k // 4096 + 2) * 2.0 ** -24
+    x8, w8, want = _products(gpu, m, n, k, False)
+    got = gpu.linear_fp8(x8, w8, out_dtype=F32).double()
+    assert float(((got - want).norm(dim=1) / want.norm(dim=1)).max()) <= 6e-7
+    gpu.device_check()
+
+
+@pytest.mark.parametrize("m,n,k", [(1280, 2048, 1 << 18), (1280, 2047, 70000), (300, 301, 1 << 18), (20, 33, 1 << 22)])
+def test_long_bf16_sums(gpu, m, n, k):
+    """A bf16 output's chains end at 65536 (c = 2048 additions: (c + 1) / 2 * 2^-23 = 1.22e-4; one chain of 2^18 was measured
+    at 4.2e-4). A residual that cancels the sum shows its error; what is left is rounded to bf16."""
+    x8, w8, want = _products(gpu, m, n, k, True)
+    resid = (-want).to(BF16)
+    one = torch.ones((n,), dtype=BF16, device="cuda")
+    left = want + resid.double()
+    err = (1024.5 * 2.0 ** -23 + (k // 65536 + 70) * 2.0 ** -24) * want  # up to 70 parts are added up
+    for fill in (0x00, 0xFF):
+        ws = torch.full((gpu.linear_fp8_workspace_size(m, n, k, True),), fill, dtype=torch.uint8, device="cuda")
+        got = gpu.linear_fp8(x8, w8, epilogue=2, gate=one, resid=resid, workspace=ws)
+        assert ((got.double() - left).abs() <= err + 2.0 ** -8 * (left.abs() + err)).all()
+    got = gpu.linear_fp8(x8, w8)
+    assert ((got.double() - want).abs() <= err + 2.0 ** -8 * (want + err)).all()
+    gpu.device_check()
