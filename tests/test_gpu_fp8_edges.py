@@ -170,3 +170,38 @@ def test_long_bf16_sums(gpu, m, n, k):
     got = gpu.linear_fp8(x8, w8)
     assert ((got.double() - want).abs() <= err + 2.0 ** -8 * (want + err)).all()
     gpu.device_check()
+
+
+def test_a_forked_stream_in_a_captured_graph(gpu):
+    """The same inside a capture that forks to a second stream: replays give what the calls give."""
+    w8, v = gpu.quantize_fp8(_rand(2, 300, 512)), _rand(3, 512).to(BF16)
+    hold = _rand(1, 400, 512).to(BF16)
+    side = torch.cuda.Stream()
+
+    def step(fork):
+        s = None
+        q = gpu.quantize_fp8(hold)
+        if fork:
+            s = side
+            side.wait_stream(torch.cuda.current_stream())
+        y = gpu.linear_fp8(q, w8, stream=s)
+        n = gpu.layernorm_train(hold, shift=v, scale=v, stream=s)
+        del q
+        back = [gpu.quantize_fp8(hold * i) for i in (2.0, 3.0)]  # of the freed size, on the first stream
+        if fork:
+            torch.cuda.current_stream().wait_stream(side)
+        return [y, *n] + [gpu.dequantize_fp8(b) for b in back]
+
+    step(False)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(True)
+    for seed in (4, 5):
+        hold.copy_(_rand(seed, 400, 512))
+        want = step(False)
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+    gpu.device_check()
