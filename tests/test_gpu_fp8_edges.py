@@ -2,6 +2,8 @@
 fp32's range, long sums, sizes beyond 32 bits, temporaries of a call on another stream."""
 from __future__ import annotations
 
+import math
+
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -204,4 +206,28 @@ def test_a_forked_stream_in_a_captured_graph(gpu):
             graph.replay()
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(got, want))
+    gpu.device_check()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("m,n,k", [(3, 24, 128), (16, 64, 300), (40, 64, 256), (300, 64, 4000)])
+def test_gelu_of_large_values(gpu, m, n, k, dtype):
+    """GELU beside values of any size: below -7.45, where its exact value is between -1e-17 and 0, nothing but that; the value
+    itself where it is large; NaN alone. Bar of the ordinary columns between them: as in the linear layers' tests."""
+    x8, w8 = gpu.quantize_fp8(_rand(1, m, k)), gpu.quantize_fp8(_rand(2, n, k) / k ** 0.5)
+    bias = _rand(3, n).to(BF16)
+    large = torch.tensor([-20.0, -1e4, -1e20, -3e38, 20.0, 1e4, 1e20, 3e38], device="cuda").to(BF16)
+    bias[1::8] = large[:n // 8]
+    bias[6::8] = float("nan")
+    got = gpu.linear_fp8(x8, w8, bias, epilogue=1, out_dtype=dtype).double()
+    y, size = ref.linear(*(gpu.dequantize_fp8(t, dtype=F32).double() for t in (x8, w8)), bias)
+    want = torch.where(y.abs() > 30, y.clamp(min=0.0), y / (1.0 + torch.exp(-2.0 * (2.0 / math.pi) ** 0.5 * (y + 0.044715 * y ** 3))))
+    cols = torch.arange(n, device="cuda")
+    assert got[:, cols % 8 == 6].isnan().all() and not got[:, cols % 8 != 6].isnan().any()
+    far = (y < -7.45) & ~y.isnan()
+    assert far.any() and (got[far].abs() <= 1.01e-17).all()
+    near = ~far & ~y.isnan()
+    bar = 1.13 * (k + 8) * 2.0 ** -23 * size + 2.0 ** -20 * want.abs()
+    bar = bar + torch.finfo(dtype).eps / 2 * (want.abs() + bar)
+    assert ((got - want).abs() <= bar)[near].all()
     gpu.device_check()
