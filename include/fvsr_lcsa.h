@@ -352,9 +352,11 @@ fvsr_status fvsr_cross_attention(int32_t heads, int32_t lq, int32_t lk, const vo
  * fvsr_quantize_fp8 — x (rows, cols), dtype FVSR_BF16 or FVSR_F32, into its form (q, scale) and / or the form of its
  * transpose, a (cols, rows) tensor (qt, scale_t); a pair may be NULL, not both. square = 0: one scale for each row's
  * block (of x for q, of its transpose for qt); 1: one for each 128 x 128 square of x, the same for both forms (weights).
- * fvsr_dequantize_fp8 — the values back as bf16 or fp32 (rounded once; exact unless below bf16's / fp32's range).
+ * fvsr_dequantize_fp8 — the values back as bf16 or fp32 (rounded once; exact unless outside bf16's / fp32's range).
  * rows >= 0, 1 <= cols, rows and cols at most 2^30, rows * cols at most 2^40. 16-byte alignment for x, q, qt and the
- * scales; 4-byte for the tensor read back into. */
+ * scales; 4-byte for the tensor read back into. These calls, the linear layers and the norms below read tensors whose rows
+ * do not start or end on 16 bytes by the aligned 16-byte words that hold them: up to 14 bytes beside a tensor, never beyond
+ * the word its first or last byte is in, are read and not used. Nothing beside a tensor is written. */
 fvsr_status fvsr_fp8_bytes(int64_t rows, int64_t cols, size_t* value_bytes, size_t* scale_bytes);
 fvsr_status fvsr_fp8_codes(int64_t rows, int64_t cols, const void* scale, void* out, fvsr_stream_t stream);
 fvsr_status fvsr_quantize_fp8(int64_t rows, int64_t cols, const void* x, int32_t dtype, int32_t square, void* q,
@@ -392,8 +394,8 @@ fvsr_status fvsr_linear_fp8(int32_t m, int32_t n, int32_t k, const void* x, cons
  * fvsr_layernorm_backward — dx and the vectors' gradients (fp32, (c); each may be NULL) from dy, mean and rstd and the
  * input x: in dtype with x_scale NULL, or in the 8-bit form. With g = dy * (1 + scale) * weight: dx = rstd * (g -
  * mean_c(g) - n * mean_c(g * n)); dweight = (1 + scale) * sum(dy * n), dbias = (1 + scale) * sum(dy), dscale =
- * sum(dy * (n * weight + bias)), dshift = sum(dy), sums over the rows in a fixed order (the same bits each time). dx may
- * be dy. weight, bias and scale as in the forward pass (shift is not needed). workspace:
+ * sum(dy * (n * weight + bias)), dshift = sum(dy), sums over the rows in a fixed order (the same bits each time for the same
+ * shape, types and offsets of dy, x and dx from 16 bytes on the same device; those choose the order). dx may be dy. weight, bias and scale as in the forward pass (shift is not needed). workspace:
  * fvsr_layernorm_backward_workspace_size bytes, 16-byte aligned, for this call alone until it is done. With m = 0 the
  * vectors' gradients are zero. Alignment: a row-major tensor needs its element's (8-bit values and scales: 16). */
 fvsr_status fvsr_layernorm_train(int64_t m, int32_t c, const void* x, int32_t dtype, const void* weight,

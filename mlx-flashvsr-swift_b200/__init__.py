@@ -715,7 +715,9 @@ def cross_attention(q, k, v, heads: int, out=None, stream=None):
 
 
 # ---------------------------------------------------------------------------------------------------------------
-# 8-bit tensors, the linear layers on them, LayerNorm for training
+# 8-bit tensors, the linear layers on them, LayerNorm for training. As all of this module's calls they are opaque to
+# autograd: what they return is detached, whether an input requires a gradient or not, and the backward calls are made by
+# the caller.
 # ---------------------------------------------------------------------------------------------------------------
 
 class Fp8Tensor:
@@ -906,7 +908,8 @@ def linear_fp8(x, w: Fp8Tensor, bias=None, epilogue: int = FVSR_LINEAR, gate=Non
     (N, K) an Fp8Tensor; bias, gate (N) bf16; the epilogues of `linear` in fp32 with one rounding. out (M, N) bf16 (the
     default) or fp32, resid like out. Input gradient: linear_fp8(dy, w_t) with w_t the transposed form of the weight;
     weight gradient: linear_fp8(dy_t, x_t, out_dtype=torch.float32) with the transposed forms of dy and x. workspace:
-    a uint8 tensor of linear_fp8_workspace_size(...) bytes, else it is allocated."""
+    a uint8 tensor of linear_fp8_workspace_size(...) bytes, else it is allocated. Not recorded by autograd. The epilogues
+    have no backward call: a step that needs their gradients takes FVSR_LINEAR and applies them itself."""
     torch = _torch()
     held = isinstance(x, Fp8Tensor)
     xt = x.data if held else _matrix(x, "x", dtypes=(torch.bfloat16,))
@@ -951,7 +954,7 @@ def linear_fp8_workspace_size(m: int, n: int, k: int, x_is_fp8: bool) -> int:
 def layernorm_train(x, weight=None, bias=None, shift=None, scale=None, eps: float = 1e-6, out=None, stream=None):
     """LayerNorm's forward pass for training (fvsr_layernorm_train): (out, mean, rstd) with n = (x - mean) * rstd and
     out = (n * weight + bias) * (1 + scale) + shift; x (M, C) bf16 or fp32, the vectors (C) like x, mean and rstd (M)
-    fp32 for layernorm_backward."""
+    fp32 for layernorm_backward. Not recorded by autograd: the caller calls layernorm_backward."""
     x = _matrix(x, "x")
     away = _elsewhere(x, stream, x, weight, bias, shift, scale, out)
     if away is not None:

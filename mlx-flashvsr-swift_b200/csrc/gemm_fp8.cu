@@ -26,7 +26,7 @@
 // tile's MMAs start some hundred cycles into the epilogue and run beside the rest of it.
 // The epilogue's signals that an accumulator is free carry no release at cluster scope, which waited for its stores (a
 // tile took 1900 cycles longer: 162 instead of 138 us below).
-// Measured from 8-bit operands at the full clock (zeros): 17280 × 8960 × 1536 138 us = 3442 TFLOP/s, with GELU 149;
+// Measured on operands of zeros, which leave the clock at its highest: 17280 × 8960 × 1536 138 us = 3442 TFLOP/s, with GELU 153;
 // 17280 × 1536 × 8960 129 us = 3694. 4 stages 151, 150 and 148 us; groups of 8 tile rows 146, 152 and 130. On random
 // values the clock falls to 1.5 GHz at 1000 W and energy decides: 180 us = 2644 TFLOP/s, 195 and (gated) 183.
 // Not kept, measured before the two lines above held: 256 × 384 tiles in two accumulators of 192 columns, and sixteen

@@ -7,8 +7,8 @@
 // (m16n8k16: 16 rows of w against 8 tokens, fp32 sums); which of a block's 128 positions an instruction's k index means
 // does not matter as long as both operands agree, so a lane reads 16 consecutive bytes of a row and uses them as they
 // come. Each block's sum is scaled by its two powers of two and added in fp32; the warps' sums are added in order.
-// One B200, from bf16: 1 × 9216 × 1536 6.8 µs, 16 tokens 9.1 (17 tokens on the tiled kernel: 7.7 from 8-bit x, and 2 to
-// quantise it); 1 × 1536 × 1536 3.2, 16 tokens 5.0 (17: 7.4 and 2). Hence the limit of 16.
+// One B200, from bf16: 1 × 9216 × 1536 6.8 µs, 16 tokens 9.2 (17 tokens on the tiled kernel: 7.7 from 8-bit x, and 2 to
+// quantise it); 1 × 1536 × 1536 3.4, 16 tokens 5.0 (17: 7.5 and 2). Hence the limit of 16.
 #include "../../include/fvsr_lcsa.h"
 #include "common.cuh"
 #include "fp8.cuh"

@@ -5,7 +5,7 @@
 //   A = Σ_rows dy·n, B = Σ_rows dy: dw = (1 + scale)·A, db = (1 + scale)·B, dscale = w·A + b·B, dshift = B.
 // fp32 throughout, one rounding of y and dx to the tensors' type.
 //
-// Both passes are bound by memory, x (and dy) read once and the result written once. A thread owns eight channels (or
+// Both passes move bytes, x (and dy) read once and the result written once. A thread owns eight channels (or
 // twice eight) of every row it meets, so the vectors, and in the backward pass the sums A and B of those channels, stay in
 // its registers over all rows: tpr = ⌈c / 8⌉ threads, in whole warps, work on a row, kRows rows at once to share a
 // barrier; narrow rows put several such groups in a CTA. Rows are copied ahead into shared memory with cp.async, each
@@ -19,11 +19,15 @@
 //   17,280 × 1536 bf16                               22 (0.73)   37 (0.66)   40
 //   30,720 × 1536 bf16                               34 (0.84)   55 (0.79)   60
 //   4096 × 8192 bf16                                 28 (0.74)   54 (0.57)   56
-//   17,280 × 1536 fp32                               39 (0.83)   58 (0.85)   45
-//   17,280 × 1531 bf16                               33          46          67
-//   17,280 × 1531 fp32                               38          63          81
-// What keeps the backward pass in bf16 from memory's rate is instructions: 152 for a thread's eight values of a row (194
-// from 8 bits); off the grid the warps with a row's ends have the more of them that the row's other warps wait for.
+//   17,280 × 1536 fp32                               39 (0.83)   57 (0.85)   45
+//   8640 × 2048 bf16                                 17 (0.64)   28 (0.57)   29
+//   4096 × 8192 bf16                                 28 (0.74)   55 (0.57)   57
+//   17,280 × 1531 bf16                               33          45          66
+//   17,280 × 1531 fp32                               38          62          73
+// What keeps bf16 from memory's rate is neither memory nor instructions, but waits: at 17,280 × 1536 the backward pass has
+// DRAM 45 % busy (from 8 bits 32 %, the forward pass 30 %) and half of its issue slots used, by 15 warps an SM (21) that its
+// registers leave, which wait for their own results, for shared memory and for the barrier of every two rows. The CTAs
+// divide an SM's registers evenly at 1536 channels; at 2048 and above 4096 fewer warps share it.
 #include "../../include/fvsr_lcsa.h"
 #include "common.cuh"
 #include "fp8.cuh"

@@ -15,7 +15,9 @@
 // One B200, bf16 (share of the copy rate, 6533 GB/s): 30,720 × 1536 to rows 23.7 µs (0.91), to both forms 38.0 (0.76), back
 // 23.9 (0.91); at 17,280 rows 14.5, 20.4 and 13.7. Reading the tile by columns for the transposed bf16 form took 25.1
 // instead of 20.4, a dequantising lane that owns 32 consecutive output bytes 19.3 instead of 13.7. Rows off the 16-byte grid
-// (17,280 × 1531) to rows 20.6, to both forms 29.3, back 24: shifts, and sectors that two accesses share.
+// (17,280 × 1531) to rows 20.6, to both forms 29.3, back 24: shifts, and sectors that two accesses share. fp32, 17,280 × 1536:
+// to rows 31 (0.65), to both forms 38 (0.64), back 22 (0.92); its pieces are four values, and 64 KB of tile and the columns
+// held in registers leave the transposed form three CTAs an SM.
 #include <type_traits>
 
 #include "../../include/fvsr_lcsa.h"
